@@ -561,6 +561,54 @@ int tad_flip_categories(int64_t rows, int64_t F, int n_cols, const int32_t* cols
                         const float* cond, int64_t ld, const float* rnd, const int64_t* base_draw, float p, float* out,
                         int64_t ldo, tad_stream_t stream);
 
+/* ------------------------------------------------------------------ token family
+ * The two ends of a discrete column whose codes are integers: the lookup of a code's row with its gradient, a loss on a
+ * code's logits against a teacher's, and the draw of a code from its logits.  No counterparts in the reference (its
+ * nn.Embedding on float codes is tad_embed_fwd / tad_embed_bwd, its decoder takes the argmax: tad_heads_to_tensor).
+ * Tokens and indices are int64. */
+
+/* out[i, :] = scale * table[tokens[i * tok_stride], :], i < n; table [vocab, D] and out [n, D] float32 or bf16 (table_dtype,
+ * out_dtype), any row strides >= D (16-byte aligned bases and D, ld multiples of 8 (both bf16) or 4 move 16 bytes a lane).
+ * A token outside [0, vocab) is padding: its row of out is zeros.  The product is formed in float32 and rounded once. */
+int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, int64_t tok_stride, float scale, const void* table,
+                        int table_dtype, int64_t ld_table, void* out, int out_dtype, int64_t ldo, tad_stream_t stream);
+/* Its gradient: dtable[v, :] = (accumulate: +=) scale * sum over the i with tokens[i * tok_stride] = v of dout[i, :]; dout
+ * [n, D] float32 or bf16, dtable [vocab, D] float32.  Without accumulate every row of dtable is written (zeros where no token
+ * names it); with it the rows that no token names are not touched.  Padding tokens have no share.  The sums are float32 in a
+ * fixed order (tokens sorted, equal ones by position): the same bits from every call.  n < 2^31, vocab < 2^31 - 1.
+ * workspace: tad_token_embed_bwd_workspace_bytes(n, D) bytes, 16-byte aligned, not read before it is written; calls that
+ * overlap on the device (and graphs that may) need workspaces of their own. */
+int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D);
+int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, int64_t tok_stride, float scale, const void* dout,
+                        int dout_dtype, int64_t ld_dout, float* dtable, int64_t ld_dtable, int accumulate, void* workspace,
+                        int64_t workspace_bytes, tad_stream_t stream);
+
+/* Distillation from a teacher's K top logits per row (1 <= K <= 1024), loss and gradient:
+ *   q_k = softmax over the row's entries of value[r, k] / tau;  an index outside [0, V) is no entry, an index that comes
+ *   twice has the sum of its q;  p_j = softmax of logits[r, j] / tau;  w_r = row_weight[r] (NULL: 1)
+ *   loss_rows[r]  = w_r tau^2 sum_k q_k (ln q_k - ln p[index_k])
+ *   dlogits[r, j] = grad_scale * d loss_rows[r] / d logits[r, j] = grad_scale w_r tau (p_j - q of j)
+ * logits and dlogits [rows, V] of `dtype`, index int64 and value float32 [rows, K] (row stride ld_t).  dlogits may be NULL
+ * (the loss alone) or the logits' own storage (same row stride).  Statistics and sums are float32.  The loss and the gradient
+ * of a row are 0 where its weight is 0 (whatever else it holds), where it has no entry with a value above -inf, and where no
+ * student logit is above -inf.  A logit of -inf has p = 0; q above 0 there makes the row's loss +inf. */
+int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dtype, int64_t ld, const int64_t* index, const float* value,
+                     int64_t ld_t, float tau, const float* row_weight, float grad_scale, float* loss_rows, void* dlogits, int64_t ldd,
+                     tad_stream_t stream);
+
+/* A token from each row of logits [rows, V] (float32 or bf16) with the uniform number u[r] in [0, 1):
+ *   w_j = exp((l_j - max l) / T);  kept: the top_k largest (0: all); of those the shortest prefix, largest first, whose mass
+ *   is at least top_p of theirs (1 or more: all; at least one is kept); of those the ones with w_j >= min_p (0: all);
+ *   out[r] = the lowest index j at which the sum of the kept w up to j exceeds u[r] times the sum of all kept w.
+ * Ties go to the lowest index.  T = 0 takes the largest logit.  -inf and NaN logits are never drawn; a row with no other
+ * gives -1; among +inf logits the draw is even.  Each setting is one number, or, where its _rows pointer is given, a number
+ * per row (T, top_p, min_p float32, top_k int32; there T not above 0 means 0, top_k below 1 means all, min_p above 1 means 1;
+ * NaN: T 0, the others off).  u below 0 or NaN counts as 0, u of 1 or more gives the last kept token.  The masses are
+ * integers, multiples of 2^-44 of the largest weight (fewer bits from 2^18 logits on): every sum is exact. */
+int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, int dtype, int64_t ld, double temperature, const float* temperature_rows,
+                      int64_t top_k, const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
+                      const float* min_p_rows, const float* u, int64_t* out, tad_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

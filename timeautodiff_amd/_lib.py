@@ -17,6 +17,7 @@ _p = C.c_void_p
 _i64 = C.c_int64
 _i = C.c_int
 _f = C.c_float
+_d = C.c_double
 
 
 class RnnDir(C.Structure):
@@ -124,6 +125,11 @@ PROTOTYPES = {
     "tad_metadata_noise": (_i, [_i64, _i64, _i, C.POINTER(C.c_int32), _p, _i64, _p, _f, _p, _p, _i64, _p]),
     "tad_metadata_noise_static": (_i, [_i64, _i64, _i, C.POINTER(C.c_int32), _p, _i64, _p, _f, _p, _i64, _p]),
     "tad_flip_categories": (_i, [_i64, _i64, _i, C.POINTER(C.c_int32), C.POINTER(C.c_int32), _p, _i64, _p, _p, _f, _p, _i64, _p]),
+    "tad_token_embed_fwd": (_i, [_i64, _i, _i64, _p, _i64, _f, _p, _i, _i64, _p, _i, _i64, _p]),
+    "tad_token_embed_bwd_workspace_bytes": (_i64, [_i64, _i]),
+    "tad_token_embed_bwd": (_i, [_i64, _i, _i64, _p, _i64, _f, _p, _i, _i64, _p, _i64, _i, _p, _i64, _p]),
+    "tad_distill_loss": (_i, [_i64, _i64, _i, _p, _i, _i64, _p, _p, _i64, _f, _p, _f, _p, _p, _i64, _p]),
+    "tad_sample_tokens": (_i, [_i64, _i64, _p, _i, _i64, _d, _p, _i64, _p, _d, _p, _d, _p, _p, _p, _p]),
     "tad_heads_to_tensor": (_i, [_i64, _i, _i, _i, C.POINTER(C.c_int32), _p, _i64, _p, _i64, _p]),
 }
 

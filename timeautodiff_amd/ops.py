@@ -301,6 +301,12 @@ def _dt(t):
     return BF16 if t.dtype == torch.bfloat16 else F32
 
 
+def _dtype(t):
+    """The element type of a tensor as the C ABI names it (float32 and bfloat16 only)."""
+    assert t.dtype in (torch.float32, torch.bfloat16), t.dtype
+    return BF16 if t.dtype == torch.bfloat16 else F32
+
+
 def _sfx(out):
     """Entry-point suffix by the element type of a result: '' float32, '_b16' bfloat16."""
     assert out.dtype in (torch.float32, torch.bfloat16), out.dtype
@@ -932,3 +938,91 @@ def heads_to_tensor(heads, nb, nc, nn, cards, out):
     assert rows == rows2 and F == nb + nc + nn and NH == nb + sum(cards[:nc]) + nn, (heads.shape, out.shape)
     _call("tad_heads_to_tensor", rows, nb, nc, nn, _i32(list(cards)) if nc else None, hp, ldh, op, ldo, _stream(),
           cost=(0.0, 4.0 * rows * (NH + F)))
+
+
+# ------------------------------------------------------------------ token family
+def _vec(t, dtype):
+    """(ptr, n, stride) of a 1-D tensor (any stride), or of a contiguous one of any shape taken as 1-D."""
+    _chk_dev(t)
+    assert t.dtype == dtype, (t.dtype, dtype)
+    if t.dim() == 1:
+        return t.data_ptr(), t.shape[0], t.stride(0)
+    assert t.is_contiguous(), (t.shape, t.stride())
+    return t.data_ptr(), t.numel(), 1
+
+
+def token_embed_fwd(tokens, table, out, scale=1.0):
+    """out[i] = scale * table[tokens[i]]: tokens int64 (1-D of any stride, or contiguous), table [V, D] and out [..., D] float32
+    or bfloat16.  A token outside [0, V) is padding: a row of zeros."""
+    kp, n, ks = _vec(tokens, torch.int64)
+    assert table.dim() == 2
+    tp, V, D, ldt = as2d(table, table.dtype)
+    op, rows, Do, ldo = as2d(out, out.dtype)
+    assert rows == n and D == Do, (tokens.shape, table.shape, out.shape)
+    _call("tad_token_embed_fwd", n, D, V, kp, ks, float(scale), tp, _dtype(table), ldt, op, _dtype(out), ldo, _stream(),
+          cost=(float(n * D), 8.0 * n + min(n, V) * D * table.element_size() + n * D * out.element_size()))
+
+
+def token_embed_bwd_workspace_bytes(n, D):
+    """Device memory a call of token_embed_bwd for n tokens of D columns works in."""
+    return _lib.load().tad_token_embed_bwd_workspace_bytes(n, D)
+
+
+def token_embed_bwd(tokens, dout, dtable, scale=1.0, accumulate=True, workspace=None):
+    """Gradient of token_embed_fwd by sorted tokens: dtable[v] += scale * sum of dout[i] over the i with tokens[i] = v, in a
+    fixed order; accumulate=False writes every row of dtable instead (zeros where no token names it).  dout [..., D]
+    float32 or bfloat16, dtable [V, D] float32.  workspace: a uint8 tensor of token_embed_bwd_workspace_bytes(...) bytes that no
+    other call in flight uses (default: allocated for the call)."""
+    kp, n, ks = _vec(tokens, torch.int64)
+    dp, rows, D, ldd = as2d(dout, dout.dtype)
+    assert dtable.dim() == 2
+    gp, V, Dg, ldg = as2d(dtable)
+    assert rows == n and D == Dg, (tokens.shape, dout.shape, dtable.shape)
+    if workspace is None:
+        workspace = torch.empty(token_embed_bwd_workspace_bytes(n, D), dtype=torch.uint8, device=dtable.device)
+    assert workspace.dtype == torch.uint8 and workspace.is_contiguous()
+    _call("tad_token_embed_bwd", n, D, V, kp, ks, float(scale), dp, _dtype(dout), ldd, gp, ldg, int(bool(accumulate)), _ptr(workspace),
+          workspace.numel(), _stream(), cost=(float(n * D), 8.0 * n + n * D * dout.element_size() + 4.0 * D * (2 * min(n, V) if accumulate else V)))
+
+
+def distill_loss(logits, index, value, loss_rows, temperature=1.0, row_weight=None, grad_scale=1.0, dlogits=None):
+    """Distillation from a teacher's top logits: loss_rows[r] = w_r tau^2 KL(q || p), q the softmax of value[r] / tau over the
+    entries whose index lies in [0, V), p the softmax of logits[r] / tau; dlogits (optional; may be logits itself) =
+    grad_scale * the gradient.  logits / dlogits [..., V] float32 or bfloat16, index int64 and value float32 [..., K],
+    row_weight and loss_rows contiguous float32 of one number per row."""
+    xp, rows, V, ld = as2d(logits, logits.dtype)
+    ip, ri, K, ldi = as2d(index, torch.int64)
+    vp, rv, Kv, ldv = as2d(value)
+    assert ri == rows and rv == rows and K == Kv and (ldi == ldv or rows == 1), (logits.shape, index.shape, index.stride(), value.shape, value.stride())
+    assert loss_rows.dtype == torch.float32 and loss_rows.is_contiguous() and loss_rows.numel() == rows
+    assert row_weight is None or (row_weight.dtype == torch.float32 and row_weight.is_contiguous() and row_weight.numel() == rows)
+    dp, ldd = None, 0
+    if dlogits is not None:
+        dp, rd, Vd, ldd = as2d(dlogits, logits.dtype)
+        assert rd == rows and Vd == V, (logits.shape, dlogits.shape)
+    _call("tad_distill_loss", rows, V, K, xp, _dtype(logits), ld, ip, vp, max(ldi, K), float(temperature), _ptr(row_weight), float(grad_scale),
+          _ptr(loss_rows), dp, ldd, _stream(), cost=((6.0 if dp else 3.0) * rows * V, rows * (V * logits.element_size() * (2.0 if dp else 1.0) + 12.0 * K + 8.0)))
+
+
+def _setting(v, rows, dtype):
+    """A setting of sample_tokens: (number, None), or (0, pointer) for a tensor of one number per row."""
+    if not isinstance(v, torch.Tensor):
+        return v, None
+    assert v.dtype == dtype and v.is_contiguous() and v.numel() == rows, (v.dtype, v.shape, rows)
+    return 0, _ptr(v)
+
+
+def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """out[r] = a token drawn from softmax(logits[r] / temperature) cut to its top_k largest (0: off), of those to the shortest
+    prefix that holds top_p of their mass (1: off), of those to the ones of at least min_p times the largest's (0: off), with
+    the uniform number u[r]; see tad_sample_tokens for ties, masked rows (-1) and the order of the sum.  logits [..., V]
+    float32 or bfloat16, u float32 and out int64, contiguous.  Each setting is a number or a tensor of one number per row
+    (float32; top_k int32)."""
+    xp, rows, V, ld = as2d(logits, logits.dtype)
+    assert u.dtype == torch.float32 and u.is_contiguous() and u.numel() == rows and out.dtype == torch.int64 and out.is_contiguous() and out.numel() == rows
+    T, Tp = _setting(temperature, rows, torch.float32)
+    k, kp = _setting(top_k, rows, torch.int32)
+    p, pp = _setting(top_p, rows, torch.float32)
+    m, mp = _setting(min_p, rows, torch.float32)
+    _call("tad_sample_tokens", rows, V, xp, _dtype(logits), ld, float(T), Tp, int(k), kp, float(p), pp, float(m), mp, _ptr(u), _ptr(out), _stream(),
+          cost=(4.0 * rows * V, rows * (V * logits.element_size() + 12.0)))
