@@ -6,7 +6,11 @@
 //
 // The answer is an index that a sum decides, so the sums are exact: every w is rounded once to a multiple of 2^-F (F = 44
 // for rows of up to 2^18 logits) and added as a 64-bit integer.  The order of additions then changes nothing, and the
-// answer is the real numbers' unless u lies within about 2^-40 of a border.
+// answer is the real numbers' unless u lies within about 2^-40 of a border.  Float64 fused multiply-adds issue at the rate
+// of float32 ones here, so such a weight costs about 20 instructions.
+//
+// Every filter keeps a prefix of the row in falling order (ties by index), so their conjunction is the shortest of the
+// prefixes: one cut (a key, and how many of those that equal it).
 #include <limits.h>
 #include <math.h>
 
@@ -26,16 +30,32 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __builtin_bit_cast(float, key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// log2 of w: (l - max) log2(e) / T
 struct Scale {
   float m;          // the row's largest logit
   double c;         // log2(e) / T
   int F;            // weights are multiples of 2^-F
 };
+// log2 of w
 __device__ __forceinline__ double log2_weight(const Scale& s, float l) { return l == s.m ? 0.0 : ((double)l - (double)s.m) * s.c; }
+// 2^t in units of 2^-F, rounded: 2^n times the series of e^z, z = ln 2 (t - n), |z| <= 0.347, whose first term left out is below
+// 2^-47; the last bits come out of the addition of 2^52
 __device__ __forceinline__ u64 fixed_weight(const Scale& s, double t) {
-  if (!(t > -64.0)) return 0;                       // (NaN: -inf / inf)
-  return (u64)(ldexp(exp2(t), s.F) + 0.5);
+  if (!(t > -48.0)) return 0;                       // (NaN: -inf / inf)
+  const double n = rint(t), z = (t - n) * 0.6931471805599453094;
+  double p = 1.0 / 479001600;
+  p = __builtin_fma(p, z, 1.0 / 39916800);
+  p = __builtin_fma(p, z, 1.0 / 3628800);
+  p = __builtin_fma(p, z, 1.0 / 362880);
+  p = __builtin_fma(p, z, 1.0 / 40320);
+  p = __builtin_fma(p, z, 1.0 / 5040);
+  p = __builtin_fma(p, z, 1.0 / 720);
+  p = __builtin_fma(p, z, 1.0 / 120);
+  p = __builtin_fma(p, z, 1.0 / 24);
+  p = __builtin_fma(p, z, 1.0 / 6);
+  p = __builtin_fma(p, z, 0.5);
+  p = __builtin_fma(p, z, 1.0);
+  p = __builtin_fma(p, z, 1.0);
+  return __builtin_bit_cast(u64, __builtin_amdgcn_ldexp(p, (int)n + s.F) + 4503599627370496.0) & 0xfffffffffffffull;
 }
 __device__ __forceinline__ u64 weight_of(const Scale& s, float l) {
   return l > -INFINITY ? fixed_weight(s, log2_weight(s, l)) : 0ull;
@@ -47,23 +67,170 @@ struct Settings {
   const float *Tr, *pr, *mr;
   const int32_t* kr;
 };
+struct RowSettings {
+  double T, p, tmin;       // tmin: log2 of min_p
+  int64_t k;
+  __device__ RowSettings(const Settings& st, int64_t r) {
+    T = st.Tr ? (double)st.Tr[r] : st.T;
+    k = st.kr ? (int64_t)st.kr[r] : st.k;
+    p = st.pr ? (double)st.pr[r] : st.p;
+    const double m = st.mr ? (double)st.mr[r] : st.minp;
+    tmin = m > 0.0 ? log2(m < 1.0 ? m : 1.0) : -INFINITY;
+  }
+};
+// the mass that a prefix has to reach, and the sum that has to be exceeded
+__device__ __forceinline__ u64 mass_needed(double p, u64 whole) {
+  const double d = ceil((p > 0.0 ? p : 0.0) * (double)whole);
+  const u64 n = d >= 1.0 ? (u64)d : 1;
+  return n < whole ? n : whole;
+}
+__device__ __forceinline__ u64 target_of(float u, u64 all) {
+  const u64 t = u > 0.f ? (u >= 1.f ? all : (u64)((double)u * (double)all)) : 0;
+  return t < all ? t : all - 1;
+}
+
+// ---------------------------------------------------------------- rows of at most 64 logits: a thread per row
+// A wave lays 64 rows down in LDS, column by column, and every lane walks its own: V steps a pass, nothing exchanged
+// between lanes.  The cut is found by taking the next largest until enough are kept.
+constexpr int SHORT_V = 64;
+
+template <typename T>
+__global__ __launch_bounds__(64) void sample_short_kernel(int64_t rows, int V, int lg, const T* __restrict__ logits, int64_t ld, Settings st, int F,
+                                                          const float* __restrict__ u, int64_t* __restrict__ out) {
+  extern __shared__ float s[];          // [V][65]
+  const int lane = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * 64;
+  const int sub = lane >> lg, c = lane & ((1 << lg) - 1), step = 64 >> lg;
+#pragma unroll 8
+  for (int i = sub; i < 64; i += step)
+    if (c < V) s[c * 65 + i] = r0 + i < rows ? (float)logits[(r0 + i) * ld + c] : -INFINITY;
+  __syncthreads();
+  const int64_t r = r0 + lane;
+  if (r >= rows) return;
+  const float* x = s + lane;
+  const RowSettings rs(st, r);
+  float m = -INFINITY;
+  int first = -1;
+#pragma unroll 8
+  for (int v = 0; v < V; ++v) {
+    const float l = x[v * 65];
+    if (l > m) { m = l; first = v; }
+  }
+  if (first < 0 || !(rs.T > 0.0)) {
+    out[r] = first;
+    return;
+  }
+  const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
+  const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
+  float cut = -INFINITY;                // kept: above `cut`, or equal to it at an index of at most `last`
+  int last = INT_MAX;
+  u64 kept = 0, whole = 0;
+  if (!by_k) {
+#pragma unroll 4
+    for (int v = 0; v < V; ++v) {
+      const float l = x[v * 65];
+      const double t = log2_weight(sc, l);
+      const u64 w = l > -INFINITY ? fixed_weight(sc, t) : 0;
+      whole += w;
+      kept += t >= rs.tmin ? w : 0;
+    }
+  }
+  for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); ++pass) {
+    const u64 need = pass == 1 ? mass_needed(rs.p, whole) : ~0ull;
+    const int most = by_k ? (int)rs.k : V;
+    u64 mass = 0;
+    kept = 0;
+    cut = INFINITY;
+    last = -1;
+    for (int n = 0; n < most && mass < need; ++n) {
+      float b = -INFINITY;
+      int at = -1;
+#pragma unroll 8
+      for (int v = 0; v < V; ++v) {
+        const float l = x[v * 65];
+        if ((l < cut || (l == cut && v > last)) && l > b) { b = l; at = v; }
+      }
+      if (at < 0) break;
+      cut = b;
+      last = at;
+      const double t = log2_weight(sc, b);
+      const u64 w = fixed_weight(sc, t);
+      mass += w;
+      if (t >= rs.tmin) kept += w;
+    }
+    whole = mass;
+  }
+  const u64 target = target_of(u[r], kept);
+  u64 run = 0;
+  for (int v = 0; v < V; ++v) {
+    const float l = x[v * 65];
+    if (!(l > cut || (l == cut && v <= last)) || !(l > -INFINITY)) continue;
+    const double t = log2_weight(sc, l);
+    if (t >= rs.tmin) run += fixed_weight(sc, t);
+    if (run > target) {
+      out[r] = v;
+      break;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- longer rows: a workgroup per row
+// A row as 16-byte pieces on the aligned grid: piece i holds the elements VEC i - a + (0 .. VEC - 1), a the row's distance
+// from the grid; the first and the last may be partly outside the row (-inf there, not loaded).
+template <typename T>
+struct Row {
+  static constexpr int VEC = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(VEC))) T pack;
+  const T* x;
+  int64_t V, np;
+  int a;
+  __device__ Row(const T* x_, int64_t V_) : x(x_), V(V_) {
+    a = (int)(((uintptr_t)x_ / sizeof(T)) & (VEC - 1));
+    np = (V + a + VEC - 1) / VEC;
+  }
+  __device__ __forceinline__ int64_t first(int64_t i) const { return i * VEC - a; }
+  __device__ __forceinline__ void load(int64_t i, float (&v)[VEC]) const {
+    const int64_t j = first(i);
+    if (j >= 0 && j + VEC <= V) {
+      const pack p = *reinterpret_cast<const pack*>(x + j);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = (float)p[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = j + e >= 0 && j + e < V ? (float)x[j + e] : -INFINITY;
+    }
+  }
+};
+
+constexpr int BINS = 768;       // of log2 w, sixteen to the octave, down to 2^-48
 
 template <int NT>
 struct RowState {
-  u64 mass[256];
+  static constexpr int NW = NT / 64;
+  static constexpr int CAP = NT < 256 ? 256 : NT;       // candidates
+  u64 list[CAP];
+  u64 mass[BINS];
   uint32_t cnt[256];
-  u64 wsum[NT / 64];
-  uint32_t wcnt[NT / 64];
-  uint32_t key;         // what the last descent found
-  u64 above;            // mass above that key
-  uint32_t n_above;     // number above that key
-  u64 total;
-  int64_t answer;
+  u64 wsum[NW];
+  uint32_t wcnt[NW];
+  uint32_t n, key, n_above;
+  u64 above;
 };
 
-// exclusive scan of a thread's value over the workgroup; total to *sum
 template <int NT, typename I>
-__device__ I block_scan(I v, I* s, I* sum) {
+__device__ __forceinline__ I block_total(I v, I* s) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (NT == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  I all = 0;
+  for (int w = 0; w < NT / 64; ++w) all += s[w];
+  return all;
+}
+// exclusive scan of a thread's value over the workgroup; the total to *sum
+template <int NT, typename I>
+__device__ __forceinline__ I block_scan(I v, I* s, I* sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   I inc = v;
   for (int o = 1; o < 64; o <<= 1) {
@@ -82,153 +249,382 @@ __device__ I block_scan(I v, I* s, I* sum) {
   return before + inc - v;
 }
 
-// One workgroup per row; the ordered keys are searched byte by byte, the row read once for each byte.
+// sorts list[0 .. P), P a power of two: falling, or rising
+template <int NT>
+__device__ void sort_list(u64* list, int P, bool falling) {
+  for (int size = 2; size <= P; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < P / 2; i += NT) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const u64 a = list[lo], b = list[hi];
+        if ((a < b) == (((lo & size) == 0) == falling) && a != b) { list[lo] = b; list[hi] = a; }
+      }
+    }
+  __syncthreads();
+}
+__device__ __forceinline__ int pow2_at_least(int n) {
+  int P = 64;
+  while (P < n) P <<= 1;
+  return P;
+}
+
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V, const T* __restrict__ logits, int64_t ld, Settings st, int F,
                                                         const float* __restrict__ u, int64_t* __restrict__ out) {
-  __shared__ RowState<NT> S;
-  const int tid = threadIdx.x;
+  typedef RowState<NT> State;
+  constexpr int VEC = Row<T>::VEC, NW = State::NW, CAP = State::CAP;
+  __shared__ State S;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
-  const T* x = logits + r * ld;
-  const double temp = st.Tr ? (double)st.Tr[r] : st.T;
-  const int64_t kk = st.kr ? (int64_t)st.kr[r] : st.k;
-  const double p = st.pr ? (double)st.pr[r] : st.p;
-  const double mp = st.mr ? (double)st.mr[r] : st.minp;
+  const Row<T> row(logits + r * ld, V);
+  const RowSettings rs(st, r);
+  // a wave's own contiguous share of the pieces
+  const int64_t seg = (row.np + NW - 1) / NW, lo = wave * seg < row.np ? wave * seg : row.np, hi = lo + seg < row.np ? lo + seg : row.np;
 
-  // the largest logit, and its lowest index
-  u64 best = 0;
-  for (int64_t j = tid; j < V; j += NT) {
-    const u64 b = ((u64)key_of((float)x[j]) << 32) | (uint32_t)~(uint32_t)j;
-    best = b > best ? b : best;
+#define EACH_PIECE(...)                                   \
+  _Pragma("unroll 4") for (int64_t i = lo + lane; i < hi; i += 64) { \
+    float v[VEC];                                         \
+    row.load(i, v);                                       \
+    __VA_ARGS__                                           \
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 b = __shfl_xor(best, o);
-    best = b > best ? b : best;
+
+  // the largest logit of the thread, then of the row
+  float tm = -INFINITY;
+  EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) tm = v[e] > tm ? v[e] : tm;)
+  float m = tm;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if constexpr (NT > 64) {
+    float* f = reinterpret_cast<float*>(S.wcnt);
+    if (lane == 0) f[wave] = m;
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, f[w]);
+    __syncthreads();
   }
-  if ((tid & 63) == 0) S.wsum[tid >> 6] = best;
-  __syncthreads();
-  for (int w = 0; w < NT / 64; ++w) best = S.wsum[w] > best ? S.wsum[w] : best;
-  const uint32_t kmax = (uint32_t)(best >> 32);
-  if (kmax == 0 || !(temp > 0.0)) {
-    if (tid == 0) out[r] = kmax == 0 ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+  if (m == -INFINITY) {
+    if (tid == 0) out[r] = -1;
     return;
   }
-  const Scale sc = {logit_of(kmax), 1.4426950408889634074 / temp, F};
-  const bool by_k = kk > 0 && kk < V, by_p = p < 1.0;
-  const double tmin = mp > 0.0 ? log2(mp < 1.0 ? mp : 1.0) : -INFINITY;
+  if (!(rs.T > 0.0)) {
+    u64 at = ~0ull;                       // the lowest index of the largest
+    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) if (v[e] == m) {
+      const u64 j = (u64)(row.first(i) + e);
+      at = j < at ? j : at;
+    })
+    for (int o = 32; o > 0; o >>= 1) {
+      const u64 b = __shfl_xor(at, o);
+      at = b < at ? b : at;
+    }
+    if (lane == 0) S.wsum[wave] = at;
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) at = S.wsum[w] < at ? S.wsum[w] : at;
+    if (tid == 0) out[r] = (int64_t)at;
+    return;
+  }
+  const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
+  const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
 
-  // a cut: every key above `cut`, and the first `ties` (by index) that equal it
-  uint32_t cut = 1, ties = UINT_MAX;
-  u64 whole = 0;                        // mass of what top-k keeps
-  for (int stage = by_k ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
-    // stage 0: the kk-th largest key; stage 1: the key at which the mass, from above, reaches p of the whole
-    u64 need = 0;
-    if (stage == 1) {
-      if (!by_k) {
-        u64 w = 0;
-        for (int64_t j = tid; j < V; j += NT) w += weight_of(sc, (float)x[j]);
-        block_scan<NT>(w, S.wsum, &whole);
+  // ---- few candidates: all that top-k can keep fits the list
+  if ((by_k && rs.k <= CAP / 2) || ((by_k || by_p) && V <= CAP)) {
+    const int64_t kk = by_k ? rs.k : V;
+    uint32_t thr = 0;
+    if (V > CAP) {
+      // kk threads whose largest is at least `thr`: so at least kk logits are; 16 bits of it are enough (NT < kk: no thread's
+      // largest says anything, and the list runs over)
+      const uint32_t mine = key_of(tm);
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = thr | 1u << bit;
+        int n = __popcll(__ballot(mine >= t));
+        if constexpr (NT > 64) n = __syncthreads_count(mine >= t);
+        if (n >= kk) thr = t;
       }
-      const double d = ceil((p > 0.0 ? p : 0.0) * (double)whole);
-      need = d >= 1.0 ? (u64)d : 1;
-      if (need > whole) need = whole;
     }
-    uint32_t prefix = 0;
-    u64 above = 0;
-    uint32_t n_above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      for (int b = tid; b < 256; b += NT) { S.mass[b] = 0; S.cnt[b] = 0; }
-      __syncthreads();
-      for (int64_t j = tid; j < V; j += NT) {
-        const uint32_t key = key_of((float)x[j]);
-        if (key == 0 || key < cut) continue;
-        if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-        const uint32_t b = key >> shift & 255;
-        atomicAdd(&S.cnt[b], 1u);
-        if (stage == 1 && key > cut) atomicAdd(&S.mass[b], weight_of(sc, (float)x[j]));
+    if (thr == 0) thr = 1;
+    if (tid == 0) S.n = 0;
+    __syncthreads();
+    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
+      const uint32_t key = key_of(v[e]);
+      if (key >= thr) {
+        const uint32_t at = atomicAdd(&S.n, 1u);
+        if (at < CAP) S.list[at] = (u64)key << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
       }
-      __syncthreads();
-      if (tid == 0) {
-        // the ties at top-k's own cut count only `ties` times
-        if (stage == 1 && ties != UINT_MAX && (shift == 24 || (cut >> (shift + 8)) == (prefix >> (shift + 8))))
-          S.mass[cut >> shift & 255] += ties * weight_of(sc, logit_of(cut));
-        u64 m = above;
-        uint32_t n = n_above;
-        int b = 255;
-        for (; b > 0; --b) {
-          if (stage == 0 ? n + S.cnt[b] >= (u64)kk : m + S.mass[b] >= need) break;
-          m += S.mass[b];
-          n += S.cnt[b];
-        }
-        S.key = prefix | (uint32_t)b << shift;
-        S.above = m;
-        S.n_above = n;
-      }
-      __syncthreads();
-      prefix = S.key;
-      above = S.above;
-      n_above = S.n_above;
-    }
-    if (stage == 0) {
-      // fewer than kk logits that can be drawn: the descent ends at key 0 and everything is kept
-      cut = prefix > 0 ? prefix : 1;
-      ties = prefix > 0 ? (uint32_t)(kk - n_above) : UINT_MAX;
-      u64 w = 0;
+    })
+    __syncthreads();
+    const uint32_t n = S.n;
+    if (n <= CAP) {
+      const int P = pow2_at_least((int)n);
+      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
+      sort_list<NT>(S.list, P, true);
+      const int nk = kk < n ? (int)kk : (int)n;
+      u64 whole = 0;
       if (by_p) {
-        for (int64_t j = tid; j < V; j += NT)
-          if (key_of((float)x[j]) > cut) w += weight_of(sc, (float)x[j]);
-        if (prefix == 0)
-          for (int64_t j = tid; j < V; j += NT)
-            if (key_of((float)x[j]) == cut) w += weight_of(sc, (float)x[j]);
-        block_scan<NT>(w, S.wsum, &whole);
-        if (prefix > 0) whole += ties * weight_of(sc, logit_of(cut));
+        u64 w = 0;
+        for (int i = tid; i < nk; i += NT) w += weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)));
+        whole = block_total<NT>(w, S.wsum);
       }
-    } else {
-      const u64 w = weight_of(sc, logit_of(prefix));
-      const u64 c = w ? (need - above + w - 1) / w : 1;
-      if (prefix > cut) {
+      const u64 need = by_p ? mass_needed(rs.p, whole) : ~0ull;
+      u64 above = 0, kept = 0;
+      uint32_t nkept = 0;
+      for (int base = 0; base < nk; base += NT) {
+        const int i = base + tid;
+        const double t = i < nk ? log2_weight(sc, logit_of((uint32_t)(S.list[i] >> 32))) : -INFINITY;
+        const u64 w = i < nk ? fixed_weight(sc, t) : 0;
+        u64 sum;
+        const u64 before = above + block_scan<NT>(w, S.wsum, &sum);
+        const bool keep = i < nk && before < need && t >= rs.tmin;
+        nkept += block_total<NT>((uint32_t)keep, S.wcnt);
+        kept += block_total<NT>(keep ? w : 0ull, S.wsum);
+        above += sum;
+      }
+      // by index: index << 32 | key, rising
+      const int Q = pow2_at_least((int)nkept);
+      __syncthreads();
+      for (int i = tid; i < Q; i += NT) {
+        const u64 a = S.list[i];
+        S.list[i] = i < (int)nkept ? (u64)(uint32_t)~(uint32_t)a << 32 | a >> 32 : ~0ull;
+      }
+      sort_list<NT>(S.list, Q, false);
+      const u64 target = target_of(u[r], kept);
+      u64 run = 0;
+      for (int base = 0; base < (int)nkept; base += NT) {
+        const int i = base + tid;
+        const u64 w = i < (int)nkept ? weight_of(sc, logit_of((uint32_t)S.list[i])) : 0;
+        u64 sum;
+        const u64 before = run + block_scan<NT>(w, S.wsum, &sum);
+        if (before <= target && target < before + w) out[r] = (int64_t)(S.list[i] >> 32);
+        run += sum;
+      }
+      return;
+    }
+    __syncthreads();
+  }
+
+  // ---- the cut: every key above `cut`, and the first `ties` (by index) that equal it (ALL: no need to count them)
+  constexpr uint32_t ALL = UINT_MAX;
+  uint32_t cut = 0, ties = ALL;
+  u64 whole = 0, need = 0;                 // mass of what top-k keeps, and top_p of it
+  bool found = false;
+  if (by_p && !by_k) {
+    // masses by log2 w; the bin in which the sum from above reaches what is needed is looked at closely
+    for (int b = tid; b < BINS; b += NT) S.mass[b] = 0;
+    if (tid == 0) S.n = 0;
+    __syncthreads();
+    u64 sum = 0;
+    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
+      const double t = log2_weight(sc, v[e]);
+      if (v[e] > -INFINITY && t > -48.0) {
+        const u64 w = fixed_weight(sc, t);
+        sum += w;
+        atomicAdd(&S.mass[(int)(t * -16.0)], w);
+      }
+    })
+    whole = block_total<NT>(sum, S.wsum);
+    need = mass_needed(rs.p, whole);
+    __syncthreads();
+    u64 above = 0;
+    for (int base = 0; base < BINS; base += NT) {
+      const int b = base + tid;
+      const u64 w = b < BINS ? S.mass[b] : 0;
+      u64 all;
+      const u64 before = above + block_scan<NT>(w, S.wsum, &all);
+      if (before < need && need <= before + w) { S.key = (uint32_t)b; S.above = before; }
+      above += all;
+    }
+    __syncthreads();
+    const int bin = (int)S.key;
+    above = S.above;
+    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
+      const double t = log2_weight(sc, v[e]);
+      if (v[e] > -INFINITY && t > -48.0 && (int)(t * -16.0) == bin) {
+        const uint32_t at = atomicAdd(&S.n, 1u);
+        if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+      }
+    })
+    __syncthreads();
+    const int n = (int)S.n;
+    if (S.n <= CAP) {
+      found = true;
+      const int P = pow2_at_least(n);
+      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
+      sort_list<NT>(S.list, P, true);
+      for (int base = 0; base < n; base += NT) {
+        const int i = base + tid;
+        const u64 w = i < n ? weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32))) : 0;
+        u64 all;
+        const u64 before = above + block_scan<NT>(w, S.wsum, &all);
+        if (before < need && need <= before + w) {
+          // the last one kept; how many equal it, kept and at all
+          const uint32_t key = (uint32_t)(S.list[i] >> 32);
+          int f = i, l = i;
+          while (f > 0 && (uint32_t)(S.list[f - 1] >> 32) == key) --f;
+          while (l + 1 < n && (uint32_t)(S.list[l + 1] >> 32) == key) ++l;
+          S.key = key;
+          S.n_above = l == i ? ALL : (uint32_t)(i - f + 1);
+        }
+        above += all;
+      }
+      __syncthreads();
+      cut = S.key;
+      ties = S.n_above;
+    }
+    __syncthreads();
+  }
+  if (by_k || (by_p && !found)) {
+    // many candidates, or a bin of many: the ordered keys are searched byte by byte, the row read once for each byte;
+    // stage 0: the k-th largest key; stage 1: the key at which the mass, from above, reaches what is needed
+    for (int stage = by_k ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
+      if (stage == 1) need = mass_needed(rs.p, whole);
+      uint32_t prefix = 0, n_above = 0;
+      u64 above = 0;
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int b = tid; b < 256; b += NT) { S.mass[b] = 0; S.cnt[b] = 0; }
+        __syncthreads();
+        EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
+          const uint32_t key = key_of(v[e]);
+          if (key == 0 || key < cut || (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
+          const uint32_t b = key >> shift & 255;
+          if (stage == 0) atomicAdd(&S.cnt[b], 1u);
+          else if (key > cut) atomicAdd(&S.mass[b], weight_of(sc, v[e]));
+        })
+        __syncthreads();
+        if (tid == 0) {
+          // the ties at top-k's own cut count only `ties` times
+          if (stage == 1 && ties != ALL && (shift == 24 || (cut >> (shift + 8)) == (prefix >> (shift + 8))))
+            S.mass[cut >> shift & 255] += ties * weight_of(sc, logit_of(cut));
+          u64 w = above;
+          uint32_t n = n_above;
+          int b = 255;
+          for (; b > 0; --b) {
+            if (stage == 0 ? n + S.cnt[b] >= (u64)rs.k : w + S.mass[b] >= need) break;
+            w += S.mass[b];
+            n += S.cnt[b];
+          }
+          S.key = prefix | (uint32_t)b << shift;
+          S.above = w;
+          S.n_above = n;
+        }
+        __syncthreads();
+        prefix = S.key;
+        above = S.above;
+        n_above = S.n_above;
+      }
+      if (stage == 0) {
+        // (fewer than k logits that can be drawn: the search ends at key 0 and all of them are kept)
         cut = prefix;
-        ties = c < UINT_MAX ? (uint32_t)c : UINT_MAX;
-      } else if (c < ties) {
-        ties = (uint32_t)c;
+        ties = prefix > 0 ? (uint32_t)(rs.k - n_above) : ALL;
+        if (by_p) {
+          u64 w = 0;
+          EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) if (key_of(v[e]) > cut) w += weight_of(sc, v[e]);)
+          whole = block_total<NT>(w, S.wsum);
+          if (prefix > 0) whole += ties * weight_of(sc, logit_of(cut));
+        }
+      } else {
+        const u64 w = weight_of(sc, logit_of(prefix));
+        const u64 c = w ? (need - above + w - 1) / w : 1;
+        if (prefix > cut) {
+          cut = prefix;
+          ties = c < ALL ? (uint32_t)c : ALL;
+        } else if (c < ties) {
+          ties = (uint32_t)c;
+        }
       }
     }
   }
 
-  // by index: every thread a contiguous piece; ties first, then mass, then the piece in which the sum passes
-  const int64_t seg = (V + NT - 1) / NT, lo = tid * seg < V ? tid * seg : V, hi = lo + seg < V ? lo + seg : V;
-  uint32_t eq = 0, all_eq;
-  for (int64_t j = lo; j < hi; ++j) eq += key_of((float)x[j]) == cut;
-  const uint32_t eq0 = block_scan<NT>(eq, S.wcnt, &all_eq);
-  u64 mass = 0, all;
-  uint32_t e = eq0;
-  for (int64_t j = lo; j < hi; ++j) {
-    const float l = (float)x[j];
-    const uint32_t key = key_of(l);
-    if (key < cut || key == 0 || (key == cut && e++ >= ties)) continue;
-    const double t = log2_weight(sc, l);
-    if (t >= tmin) mass += fixed_weight(sc, t);
+  // ---- by index: the waves' shares of the ties, then of the mass; the wave in whose share the sum passes walks it again
+  __syncthreads();
+  uint32_t eq = 0;                         // ties before this wave's share
+  if (ties != ALL) {
+    uint32_t n = 0;
+    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) n += key_of(v[e]) == cut;)
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    if (lane == 0) S.wcnt[wave] = n;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
   }
-  const u64 m0 = block_scan<NT>(mass, S.wsum, &all);
-  const float uu = u[r];
-  u64 target = uu > 0.f ? (u64)((double)uu * (double)all) : 0;
-  if (target >= all) target = all - 1;
-  if (m0 <= target && target < m0 + mass) {
-    u64 run = m0;
-    e = eq0;
-    for (int64_t j = lo; j < hi; ++j) {
-      const float l = (float)x[j];
-      const uint32_t key = key_of(l);
-      if (key < cut || key == 0 || (key == cut && e++ >= ties)) continue;
-      const double t = log2_weight(sc, l);
-      if (t >= tmin) run += fixed_weight(sc, t);
-      if (run > target) {
-        out[r] = j;
-        break;
+  u64 mass = 0, target = 0, run = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    uint32_t e0 = eq;
+    for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+      float v[VEC];
+      const int64_t i = i0 + lane;
+      if (i < hi) row.load(i, v);
+      else
+        for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
+      uint32_t tie = 0;                    // ties before this lane's piece
+      if (ties != ALL) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) n += key_of(v[e]) == cut;
+        uint32_t inc = n;
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint32_t up = __shfl_up(inc, o);
+          if (lane >= o) inc += up;
+        }
+        tie = e0 + inc - n;
+        e0 += __shfl(inc, 63);
       }
+      u64 w[VEC], sum = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint32_t key = key_of(v[e]);
+        w[e] = 0;
+        if (key == 0 || key < cut || (key == cut && ties != ALL && tie++ >= ties)) continue;
+        const double t = log2_weight(sc, v[e]);
+        if (t >= rs.tmin) w[e] = fixed_weight(sc, t);
+        sum += w[e];
+      }
+      if (pass == 0) {
+        mass += sum;
+        continue;
+      }
+      u64 inc = sum;
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 up = __shfl_up(inc, o);
+        if (lane >= o) inc += up;
+      }
+      u64 before = run + inc - sum;
+      if (before <= target && target < before + sum) {
+        int at = 0;
+        for (; at < VEC - 1 && before + w[at] <= target; ++at) before += w[at];
+        out[r] = row.first(i) + at;
+      }
+      run += __shfl(inc, 63);
+      if (run > target) return;
     }
+    if (pass == 1) return;
+    for (int o = 32; o > 0; o >>= 1) mass += __shfl_xor(mass, o);
+    if (lane == 0) S.wsum[wave] = mass;
+    __syncthreads();
+    u64 all = 0;
+    for (int w = 0; w < NW; ++w) {
+      if (w < wave) run += S.wsum[w];
+      all += S.wsum[w];
+    }
+    target = target_of(u[r], all);
+    if (!(run <= target && target < run + mass)) return;
   }
+#undef EACH_PIECE
+}
+
+template <typename T>
+int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const Settings& st, int F, const float* u, int64_t* out, hipStream_t s) {
+  const T* x = (const T*)logits;
+  if (V <= SHORT_V) {
+    int lg = 0;
+    while ((1 << lg) < V) ++lg;
+    hipLaunchKernelGGL(sample_short_kernel<T>, dim3((unsigned)cdiv64(rows, 64)), dim3(64), (size_t)V * 65 * 4, s, rows, (int)V, lg, x, ld, st, F, u,
+                       out);
+  } else if (V <= 2048) {
+    hipLaunchKernelGGL((sample_row_kernel<T, 64>), dim3((unsigned)rows), dim3(64), 0, s, rows, V, x, ld, st, F, u, out);
+  } else if (V <= 16384) {
+    hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, x, ld, st, F, u, out);
+  } else {
+    hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, rows, V, x, ld, st, F, u, out);
+  }
+  TAD_LAUNCH_CHECK();
+  return TAD_OK;
 }
 
 }  // namespace
@@ -250,10 +646,5 @@ extern "C" int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, in
   const int F = 62 - lg < 44 ? 62 - lg : 44;
   const Settings st = {temperature, top_p, min_p, top_k, temperature_rows, top_p_rows, min_p_rows, top_k_rows};
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == TAD_F32)
-    hipLaunchKernelGGL((sample_row_kernel<float, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, (const float*)logits, ld, st, F, u, out);
-  else
-    hipLaunchKernelGGL((sample_row_kernel<bf16_t, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, (const bf16_t*)logits, ld, st, F, u, out);
-  TAD_LAUNCH_CHECK();
-  return TAD_OK;
+  return dtype == TAD_F32 ? launch_sample<float>(rows, V, logits, ld, st, F, u, out, s) : launch_sample<bf16_t>(rows, V, logits, ld, st, F, u, out, s);
 }
