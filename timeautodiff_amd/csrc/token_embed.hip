@@ -21,8 +21,8 @@ typedef unsigned long long u64;
 
 // ---------------------------------------------------------------- element packs
 template <typename T, int VEC> struct Pack;
-template <int VEC> struct Pack<float, VEC> { typedef __attribute__((ext_vector_type(VEC))) float type; };
-template <int VEC> struct Pack<bf16_t, VEC> { typedef __attribute__((ext_vector_type(VEC))) __bf16 type; };
+template <int VEC> struct Pack<float, VEC> { typedef float type __attribute__((ext_vector_type(VEC), aligned(VEC < 4 ? 4 * VEC : 16))); };
+template <int VEC> struct Pack<bf16_t, VEC> { typedef __bf16 type __attribute__((ext_vector_type(VEC), aligned(2 * VEC))); };
 template <> struct Pack<float, 1> { typedef float type; };
 template <> struct Pack<bf16_t, 1> { typedef bf16_t type; };
 
@@ -90,66 +90,140 @@ __global__ __launch_bounds__(256) void token_embed_fwd_kernel(int64_t n, int nv,
 }
 
 // ---------------------------------------------------------------- sorting the tokens
-// key = token << 32 | position: all keys differ, and their order is the tokens' with equal ones by position.  Padding gets
-// the token `vocab`, behind every other.  A workgroup sorts a tile in LDS; tiles are merged by rank: a key's place among
-// the merged lists is its place in its own list plus, for every other list, how many of that list's keys are less (a
-// binary search): no workgroup waits for another, and no distribution of tokens is worse than another.
-constexpr int TILE = 4096;
-constexpr int FANIN = 32;     // lists merged by one launch
-
-__global__ __launch_bounds__(1024) void sort_tile_kernel(int64_t n, int64_t vocab, const int64_t* __restrict__ tok, int64_t tstride,
-                                                         u64* __restrict__ keys) {
-  __shared__ u64 s[TILE];
-  const int64_t base = (int64_t)blockIdx.x * TILE;
-  const int m = (int)(n - base < TILE ? n - base : TILE);
-  int P = 64;
-  while (P < m) P <<= 1;
-  for (int i = threadIdx.x; i < P; i += 1024) {
-    u64 k = ~0ull;
-    if (i < m) {
-      const int64_t t = tok[(base + i) * tstride];
-      k = ((u64)((uint64_t)t < (uint64_t)vocab ? t : vocab) << 32) | (u64)(base + i);
-    }
-    s[i] = k;
-  }
-  __syncthreads();
-  for (int size = 2; size <= P; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      for (int i = threadIdx.x; i < P / 2; i += 1024) {
-        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-        const u64 a = s[lo], b = s[hi];
-        if ((a > b) == ((lo & size) == 0)) { s[lo] = b; s[hi] = a; }
-      }
-      __syncthreads();
-    }
-  }
-  for (int i = threadIdx.x; i < m; i += 1024) keys[base + i] = s[i];
+// key = token << 32 | position; padding gets the token `vocab`, behind every other.  Sorted by token, equal ones by position.
+__device__ __forceinline__ u64 key_at(const int64_t* tok, int64_t tstride, int64_t vocab, int64_t i) {
+  const int64_t t = tok[i * tstride];
+  return ((u64)((uint64_t)t < (uint64_t)vocab ? t : vocab) << 32) | (u64)i;
 }
 
-// lists of `len` sorted keys each (the last one shorter), FANIN of them merged into one
-__global__ __launch_bounds__(256) void merge_rank_kernel(int64_t n, int64_t len, const u64* __restrict__ in, u64* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const u64 key = in[i];
-  const int64_t mine = i / len, first = mine / FANIN * FANIN;
-  int64_t rank = i - mine * len;
-  for (int64_t l = first; l < first + FANIN && l * len < n; ++l) {
-    if (l == mine) continue;
-    const u64* p = in + l * len;
-    int64_t lo = 0, hi = n - l * len < len ? n - l * len : len;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (p[mid] < key) lo = mid + 1; else hi = mid;
+// Up to RANK_N tokens: every token's place is counted directly, all pairs compared: a workgroup holds all tokens in LDS and
+// counts for 64 of them, each of its 16 waves over a sixteenth of the others (two instructions a comparison of 64 lanes).
+constexpr int RANK_N = 8192;
+__global__ __launch_bounds__(1024) void sort_rank_kernel(int n, int64_t vocab, const int64_t* __restrict__ tok, int64_t tstride, u64* __restrict__ keys) {
+  __shared__ __attribute__((aligned(16))) uint32_t s[RANK_N];
+  __shared__ uint32_t part[16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (n + 63) >> 6, mine = blockIdx.x;
+  for (int i = threadIdx.x; i < groups * 64; i += 1024) s[i] = i < n ? (uint32_t)(key_at(tok, tstride, vocab, i) >> 32) : UINT_MAX;
+  __syncthreads();
+  const uint32_t t = s[mine * 64 + lane];
+  uint32_t rank = 0;
+  for (int g = wave; g < groups; g += 16) {
+    const uint4* p = reinterpret_cast<const uint4*>(s + g * 64);
+    if (g != mine) {
+      const uint32_t than = t + (g < mine);        // equal ones count where they come before
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const uint4 k = p[q];
+        rank += k.x < than;
+        rank += k.y < than;
+        rank += k.z < than;
+        rank += k.w < than;
+      }
+    } else {
+      for (int q = 0; q < 64; ++q) rank += s[g * 64 + q] < t + (q < lane);
     }
-    rank += lo;
   }
-  out[first * len + rank] = key;
+  part[wave][lane] = rank;
+  __syncthreads();
+  const int i = mine * 64 + lane;
+  if (wave == 0 && i < n) {
+    for (int w = 1; w < 16; ++w) rank += part[w][lane];
+    keys[rank] = (u64)t << 32 | (u64)i;
+  }
+}
+
+// More: by digits of up to 9 bits from the lowest, two launches a digit.  A workgroup has a tile of neighbouring keys, every
+// wave a contiguous share of it, so that keys of one digit keep their order: the first launch counts digits by tile, the
+// second adds up what comes before (lower digits; earlier tiles; earlier waves) and moves the keys.  No workgroup waits for
+// another, and no distribution of tokens is worse than another.
+constexpr int MAX_BINS = 512, MAX_TILES = 64, RWAVES = 8;
+
+struct Digit {
+  const int64_t* tok;       // the first digit's source
+  int64_t tstride, vocab;
+  const u64* in;            // the others'
+  int64_t n;
+  int tile, shift, bins;
+  __device__ __forceinline__ u64 key(int64_t i) const { return in ? in[i] : key_at(tok, tstride, vocab, i); }
+  __device__ __forceinline__ int of(u64 key) const { return (int)(key >> (32 + shift)) & (bins - 1); }
+};
+
+__global__ __launch_bounds__(512) void sort_count_kernel(Digit d, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t h[MAX_BINS];
+  const int64_t base = (int64_t)blockIdx.x * d.tile;
+  const int m = (int)(d.n - base < d.tile ? d.n - base : d.tile);
+  h[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < m; i += 512) atomicAdd(&h[d.of(d.key(base + i))], 1u);
+  __syncthreads();
+  counts[blockIdx.x * MAX_BINS + threadIdx.x] = h[threadIdx.x];
+}
+
+__global__ __launch_bounds__(512) void sort_move_kernel(Digit d, int tiles, const uint32_t* __restrict__ counts, u64* __restrict__ out) {
+  __shared__ uint32_t at[RWAVES][MAX_BINS];
+  __shared__ uint32_t wsum[RWAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t base = (int64_t)blockIdx.x * d.tile;
+  const int m = (int)(d.n - base < d.tile ? d.n - base : d.tile);
+  const int share = d.tile / RWAVES, w0 = wave * share, w1 = w0 + share < m ? w0 + share : m;
+#pragma unroll
+  for (int w = 0; w < RWAVES; ++w) at[w][tid] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&at[wave][d.of(d.key(base + i))], 1u);
+  // this thread's digit: how many in all tiles, in the tiles before
+  uint32_t all = 0, before = 0;
+#pragma unroll 8
+  for (int t = 0; t < tiles; ++t) {
+    const uint32_t c = counts[t * MAX_BINS + tid];
+    all += c;
+    before += t < (int)blockIdx.x ? c : 0;
+  }
+  uint32_t inc = all;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  uint32_t place = before + inc - all;
+  for (int w = 0; w < wave; ++w) place += wsum[w];
+#pragma unroll
+  for (int w = 0; w < RWAVES; ++w) {
+    const uint32_t c = at[w][tid];
+    at[w][tid] = place;
+    place += c;
+  }
+  __syncthreads();
+  volatile uint32_t* mine = at[wave];        // this wave's alone from here on
+  for (int i0 = w0; i0 < w1; i0 += 64) {
+    const bool on = i0 + lane < w1;
+    const u64 key = on ? d.key(base + i0 + lane) : 0;
+    const int g = d.of(key);
+    u64 same = __ballot(on);
+    for (int b = 1; b < d.bins; b <<= 1) {
+      const u64 set = __ballot(g & b);
+      same &= (g & b) ? set : ~set;
+    }
+    const int ahead = __popcll(same & ((1ull << lane) - 1));
+    if (on) {
+      const uint32_t p = mine[g];
+      out[p + ahead] = key;
+      if (ahead == 0) mine[g] = p + __popcll(same);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- sums over the sorted tokens
-// A wave adds the rows of `S` neighbouring sorted positions, 64 * VEC columns of them.  A run of equal tokens that lies
-// inside the chunk is a finished row of dtable; what reaches over an edge goes to the workspace (slot 0: the run that came
-// in from the left; slot 1: one that begins here and goes on) and is added up by the launch behind.
+// A wave adds the rows of S <= 64 neighbouring sorted positions, 64 * VEC columns of them, GW waves (a chunk) side by side.
+// A run of equal tokens inside a wave's share is a finished row of dtable.  What reaches over an edge between waves of the
+// workgroup is added up in LDS, what reaches over its edges goes to the workspace (slot 0: the run that came in from the
+// left; slot 1: one that begins here and goes on) and is added up by the launch behind, always in the order of positions.
+constexpr int GW = 8;
+constexpr int ZROWS = 16;     // rows of the table a wave of the zero part looks after
+
 template <int VEC>
 __device__ __forceinline__ void put_row(float* dt, const float (&acc)[VEC], float scale, int accumulate) {
   float v[VEC];
@@ -164,19 +238,18 @@ __device__ __forceinline__ void put_row(float* dt, const float (&acc)[VEC], floa
   store_pack<float, VEC>(dt, v);
 }
 
-constexpr int ZROWS = 16;     // rows of the table a wave of the zero part looks after
-
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void embed_grad_sum_kernel(int64_t n, int D, int64_t vocab, int S, int64_t nchunks, int ctiles, float scale,
-                                                             int accumulate, const u64* __restrict__ keys, const T* __restrict__ dout, int64_t ldd,
-                                                             float* __restrict__ dtable, int64_t ldg, float* __restrict__ part) {
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t nsum = nchunks * ctiles;
-  if (w >= nsum) {
+__global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int D, int64_t vocab, int S, int64_t nchunks, int ctiles, float scale,
+                                                                 int accumulate, const u64* __restrict__ keys, const T* __restrict__ dout, int64_t ldd,
+                                                                 float* __restrict__ dtable, int64_t ldg, float* __restrict__ part) {
+  constexpr int CT = 64 * VEC, U = 8;
+  __shared__ __attribute__((aligned(16))) float edge[GW][2][CT];
+  __shared__ uint32_t head_tok[GW], tail_tok[GW], state[GW];       // state: 1 a run came in, 2 and ends here, 4 one goes on
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x >= nchunks * ctiles) {
     // rows that no token names are zero (overwriting mode): a lane looks one row up in the sorted keys
-    const int64_t v0 = (w - nsum) * ZROWS;
-    if (accumulate || v0 >= vocab) return;
+    const int64_t v0 = ((blockIdx.x - nchunks * ctiles) * GW + wave) * ZROWS;
+    if (v0 >= vocab) return;
     const int64_t v = v0 + (lane & (ZROWS - 1));
     int64_t lo = 0, hi = n;
     const u64 want = (u64)v << 32;
@@ -189,82 +262,144 @@ __global__ __launch_bounds__(256) void embed_grad_sum_kernel(int64_t n, int D, i
     for (int r = 0; r < ZROWS; ++r) {
       if (!(todo >> r & 1)) continue;
       float* row = dtable + (v0 + r) * ldg;
-      for (int c = lane * VEC; c < D; c += 64 * VEC) {
+      for (int c = lane * VEC; c < D; c += CT) {
         float z[VEC] = {};
         store_pack<float, VEC>(row + c, z);
       }
     }
     return;
   }
-  const int64_t chunk = w / ctiles;
-  const int c = (int)(w - chunk * ctiles) * 64 * VEC + lane * VEC;
-  const int64_t a = chunk * S, b = a + S < n ? a + S : n;
+  const int64_t chunk = blockIdx.x / ctiles;
+  const int c0 = (int)(blockIdx.x - chunk * ctiles) * CT, c = c0 + lane * VEC;
+  const int64_t a = (chunk * GW + wave) * S;
+  const int m = a < n ? (int)(n - a < S ? n - a : S) : 0;
   const bool on = c < D;
-  const uint32_t before = a > 0 ? (uint32_t)(keys[a - 1] >> 32) : UINT_MAX;
-  const uint32_t after = b < n ? (uint32_t)(keys[b] >> 32) : UINT_MAX;
-  float acc[VEC] = {};
-  uint32_t cur = (uint32_t)(keys[a] >> 32);
-  bool from_left = cur == before;
-  for (int64_t j = a; j < b; ++j) {
-    const u64 k = keys[j];
-    const uint32_t t = (uint32_t)(k >> 32);
-    if (t >= (uint64_t)vocab) break;                     // padding lies behind everything else
-    if (on) {
-      float v[VEC];
-      load_pack<T, VEC>(dout + (int64_t)(uint32_t)k * ldd + c, v);
+  uint32_t st = 0;
+  if (m > 0) {
+    const u64 key = keys[a + (lane < m ? lane : m - 1)];
+    const uint32_t tok = (uint32_t)(key >> 32);
+    const uint32_t left = a > 0 ? (uint32_t)(keys[a - 1] >> 32) : UINT_MAX;
+    const uint32_t right = a + m < n ? (uint32_t)(keys[a + m] >> 32) : UINT_MAX;
+    const int live = __popcll(__ballot(lane < m && tok < (uint64_t)vocab));      // padding lies behind everything else
+    uint32_t next = (uint32_t)__shfl_down(tok, 1);
+    if (lane == m - 1) next = right;
+    const u64 ends = __ballot(lane < live && tok != next);
+    const uint32_t tok0 = __builtin_amdgcn_readfirstlane(tok);
+    bool came = live > 0 && tok0 == left;
+    float acc[VEC] = {};
+    for (int j0 = 0; j0 < live; j0 += U) {
+      float v[U][VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += v[i];
-    }
-    const uint32_t next = j + 1 < b ? (uint32_t)(keys[j + 1] >> 32) : after;
-    if (next != t || j + 1 == b) {
-      if (on) {
-        if (from_left) store_pack<float, VEC>(part + (2 * chunk) * D + c, acc);
-        else if (next == t) store_pack<float, VEC>(part + (2 * chunk + 1) * D + c, acc);
-        else put_row<VEC>(dtable + (int64_t)t * ldg + c, acc, scale, accumulate);
+      for (int k = 0; k < U; ++k) {
+        const int j = j0 + k < live ? j0 + k : live - 1;             // (the last row again, not added: the loads need no branch)
+        const uint32_t pos = __builtin_amdgcn_readlane((uint32_t)key, j);
+        if (on) load_pack<T, VEC>(dout + (int64_t)pos * ldd + c, v[k]);
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-      from_left = false;
+      for (int k = 0; k < U; ++k) {
+        const int j = j0 + k;
+        if (j >= live) break;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += v[k][i];
+        if (ends >> j & 1) {
+          if (came) {
+            store_pack<float, VEC>(&edge[wave][0][lane * VEC], acc);
+            st |= 3;
+            came = false;
+          } else if (on) {
+            put_row<VEC>(dtable + (int64_t)__builtin_amdgcn_readlane(tok, j) * ldg + c, acc, scale, accumulate);
+          }
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+        }
+      }
     }
+    if (live > 0 && !(ends >> (live - 1) & 1)) {                     // goes on to the right
+      store_pack<float, VEC>(&edge[wave][came ? 0 : 1][lane * VEC], acc);
+      st |= came ? 1 : 4;
+    }
+    if (lane == 0) {
+      head_tok[wave] = tok0;
+      tail_tok[wave] = __builtin_amdgcn_readlane(tok, live > 0 ? live - 1 : 0);
+    }
+  }
+  if (lane == 0) state[wave] = st;
+  __syncthreads();
+  for (int cc = threadIdx.x; cc < CT && c0 + cc < D; cc += GW * 64) {
+    float run = 0.f;
+    bool outer = true, open = false;            // the run in hand began left of the workgroup; there is one
+    for (int w = 0; w < GW; ++w) {
+      const uint32_t f = state[w];
+      if (f & 1) {
+        run += edge[w][0][cc];
+        open = true;
+        if (f & 2) {
+          if (outer) {
+            part[(2 * chunk) * D + c0 + cc] = run;
+          } else {
+            float one[1] = {run};
+            put_row<1>(dtable + (int64_t)head_tok[w] * ldg + c0 + cc, one, scale, accumulate);
+          }
+          open = false;
+        }
+      }
+      if (f & 4) {
+        run = edge[w][1][cc];
+        outer = false;
+        open = true;
+      }
+    }
+    if (open) part[(2 * chunk + (outer ? 0 : 1)) * D + c0 + cc] = run;
   }
 }
 
 // Runs that reach over the edges of chunks: a workgroup for each chunk in which one begins (the others leave at once) and
-// each 64 columns; its waves add every fourth part, and the four sums are added in order.
-__global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, int64_t vocab, int S, int ctiles, float scale, int accumulate,
-                                                              const u64* __restrict__ keys, const float* __restrict__ part,
+// each 64 * VEC columns; its waves add every fourth part, and the four sums are added in order.
+template <int VEC>
+__global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, int64_t vocab, int P, int64_t nchunks, int ctiles, float scale,
+                                                              int accumulate, const u64* __restrict__ keys, const float* __restrict__ part,
                                                               float* __restrict__ dtable, int64_t ldg) {
+  __shared__ __attribute__((aligned(16))) float s[4][64 * VEC];
   const int64_t chunk = blockIdx.x / ctiles;
-  const int c = (int)(blockIdx.x - chunk * ctiles) * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
-  const int64_t a = chunk * S, b = a + S;
-  if (b >= n) return;
-  const uint32_t t = (uint32_t)(keys[b - 1] >> 32);
-  if (t >= (uint64_t)vocab || (uint32_t)(keys[b] >> 32) != t) return;
-  if (a > 0 && (uint32_t)(keys[a - 1] >> 32) == t) return;      // began in an earlier chunk
-  const u64 end = (u64)(t + 1) << 32;
-  int64_t lo = b, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < end) lo = mid + 1; else hi = mid;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = ((int)(blockIdx.x - chunk * ctiles) * 64 + lane) * VEC;
+  const int64_t a = chunk * P, b = a + P;                       // (not the last chunk: nothing goes on from there)
+  const uint32_t t = (uint32_t)(keys[b] >> 32);
+  if (t >= (uint64_t)vocab || (uint32_t)(keys[b - 1] >> 32) != t || (a > 0 && (uint32_t)(keys[a - 1] >> 32) == t)) return;
+  int64_t last = chunk;                                         // the last chunk that begins inside the run
+  for (bool more = true; more;) {
+    const int64_t k = last + 1 + lane;
+    const u64 in = __ballot(k < nchunks && (uint32_t)(keys[k < nchunks ? k * P : 0] >> 32) == t);
+    const int ahead = in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
+    last += ahead;
+    more = ahead == 64;
   }
-  const int64_t last = (lo - 1) / S;                             // the chunk in which the run ends
-  float acc = 0.f;
+  float acc[VEC] = {};
   if (c < D) {
-    if (wave == 0) acc = part[(2 * chunk + 1) * D + c];
-    for (int64_t k = chunk + 1 + wave; k <= last; k += 4) acc += part[(2 * k) * D + c];
+    if (wave == 0) load_pack<float, VEC>(part + (2 * chunk + 1) * D + c, acc);
+#pragma unroll 8
+    for (int64_t k = chunk + 1 + wave; k <= last; k += 4) {
+      float v[VEC];
+      load_pack<float, VEC>(part + (2 * k) * D + c, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+    }
   }
-  __shared__ float s[4][64];
-  s[wave][threadIdx.x & 63] = acc;
+  store_pack<float, VEC>(&s[wave][lane * VEC], acc);
   __syncthreads();
   if (wave == 0 && c < D) {
-    const float v = (((s[0][threadIdx.x] + s[1][threadIdx.x]) + s[2][threadIdx.x]) + s[3][threadIdx.x]) * scale;
-    float* dt = dtable + (int64_t)t * ldg + c;
-    *dt = accumulate ? *dt + v : v;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      acc[i] = ((s[0][lane * VEC + i] + s[1][lane * VEC + i]) + s[2][lane * VEC + i]) + s[3][lane * VEC + i];
+    put_row<VEC>(dtable + (int64_t)t * ldg + c, acc, scale, accumulate);
   }
 }
 
 // ---------------------------------------------------------------- host side
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+constexpr int64_t COUNT_BYTES = MAX_TILES * MAX_BINS * 4;
+inline int64_t key_bytes(int64_t n) { return (n * 8 + 15) / 16 * 16; }
 
 // How the gradient is cut: S positions a wave, VEC columns a lane.
 struct GradPlan {
@@ -280,7 +415,7 @@ GradPlan grad_plan(int64_t n, int D, int dtype, bool wide) {
   g.ctiles = (int)cdiv64(D, 64 * g.vec);
   g.S = 64;
   while (g.S > 8 && cdiv64(n, g.S) * g.ctiles < 4096) g.S /= 2;
-  g.nchunks = cdiv64(n, g.S);
+  g.nchunks = cdiv64(n, g.S * GW);
   return g;
 }
 
@@ -307,9 +442,9 @@ int launch_fwd(int64_t n, int D, int64_t vocab, const int64_t* tok, int64_t tstr
 template <typename T, int VEC>
 void launch_sum(const GradPlan& g, int64_t n, int D, int64_t vocab, float scale, int accumulate, const u64* keys, const void* dout, int64_t ldd,
                 float* dtable, int64_t ldg, float* part, hipStream_t s) {
-  const int64_t waves = g.nchunks * g.ctiles + (accumulate ? 0 : cdiv64(vocab, ZROWS));
-  hipLaunchKernelGGL((embed_grad_sum_kernel<T, VEC>), dim3((unsigned)cdiv64(waves, 4)), dim3(256), 0, s, n, D, vocab, g.S, g.nchunks, g.ctiles,
-                     scale, accumulate, keys, (const T*)dout, ldd, dtable, ldg, part);
+  const int64_t grid = g.nchunks * g.ctiles + (accumulate ? 0 : cdiv64(vocab, ZROWS * GW));
+  hipLaunchKernelGGL((embed_grad_sum_kernel<T, VEC>), dim3((unsigned)grid), dim3(GW * 64), 0, s, n, D, vocab, g.S, g.nchunks, g.ctiles, scale,
+                     accumulate, keys, (const T*)dout, ldd, dtable, ldg, part);
 }
 
 }  // namespace
@@ -329,7 +464,7 @@ extern "C" int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_
                               : launch_fwd<bf16_t, bf16_t>(n, D, vocab, tokens, tok_stride, scale, table, ld_table, out, ldo, s);
 }
 
-// keys twice (the lists and their merge), then the parts of runs over edges
+// the keys twice, the digits' counts, then the parts of runs over edges
 extern "C" int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D) {
   if (n <= 0 || D < 1) return 0;
   // the parts of the finest cut that any alignment or type of dout leads to
@@ -339,7 +474,7 @@ extern "C" int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D) {
       const GradPlan g = grad_plan(n, D, dt, wide);
       if (2 * g.nchunks * D > part) part = 2 * g.nchunks * D;
     }
-  return 2 * ((n * 8 + 15) / 16 * 16) + part * 4;
+  return 2 * key_bytes(n) + COUNT_BYTES + part * 4;
 }
 
 extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, int64_t tok_stride, float scale, const void* dout,
@@ -356,19 +491,32 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
   const bool wide = ld_dtable % 4 == 0 && D % (dout_dtype == TAD_BF16 ? 8 : 4) == 0 && ld_dout % (dout_dtype == TAD_BF16 ? 8 : 4) == 0 &&
                     aligned16(dout) && aligned16(dtable);
   const GradPlan g = grad_plan(n, D, dout_dtype, wide);
-  const int64_t kb = (n * 8 + 15) / 16 * 16;
-  TAD_CHECK(workspace && aligned16(workspace) && workspace_bytes >= 2 * kb + 2 * g.nchunks * D * 4,
+  const int64_t kb = key_bytes(n);
+  TAD_CHECK(workspace && aligned16(workspace) && workspace_bytes >= 2 * kb + COUNT_BYTES + 2 * g.nchunks * D * 4,
             "tad_token_embed_bwd: workspace of %lld bytes, 16-byte aligned, needed", (long long)tad_token_embed_bwd_workspace_bytes(n, D));
-  TAD_CHECK((g.nchunks * g.ctiles + cdiv64(vocab, ZROWS)) / 4 < INT_MAX && g.nchunks * cdiv64(D, 64) < INT_MAX, "tad_token_embed_bwd: too many tokens");
+  TAD_CHECK(g.nchunks * g.ctiles + cdiv64(vocab, ZROWS * GW) < INT_MAX && g.nchunks * cdiv64(D, 64) < INT_MAX, "tad_token_embed_bwd: too many tokens");
   u64* a = (u64*)workspace;
   u64* b = (u64*)((char*)workspace + kb);
-  float* part = (float*)((char*)workspace + 2 * kb);
-  hipLaunchKernelGGL(sort_tile_kernel, dim3((unsigned)cdiv64(n, TILE)), dim3(1024), 0, s, n, vocab, tokens, tok_stride, a);
-  TAD_LAUNCH_CHECK();
-  for (int64_t len = TILE; len < n; len *= FANIN) {
-    hipLaunchKernelGGL(merge_rank_kernel, dim3((unsigned)cdiv64(n, 256)), dim3(256), 0, s, n, len, a, b);
+  uint32_t* counts = (uint32_t*)((char*)workspace + 2 * kb);
+  float* part = (float*)((char*)workspace + 2 * kb + COUNT_BYTES);
+  if (n <= RANK_N) {
+    hipLaunchKernelGGL(sort_rank_kernel, dim3((unsigned)cdiv64(n, 64)), dim3(1024), 0, s, (int)n, vocab, tokens, tok_stride, a);
     TAD_LAUNCH_CHECK();
-    u64* t = a; a = b; b = t;
+  } else {
+    int bits = 1, tile = 2048;
+    while (vocab >> bits) ++bits;                      // tokens 0 .. vocab (padding)
+    while (cdiv64(n, tile) > MAX_TILES) tile *= 2;
+    const int digits = (bits + 8) / 9, width = (bits + digits - 1) / digits, tiles = (int)cdiv64(n, tile);
+    Digit d = {tokens, tok_stride, vocab, nullptr, n, tile, 0, 1 << width};
+    for (int k = 0; k < digits; ++k, d.shift += width) {
+      hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)tiles), dim3(512), 0, s, d, counts);
+      TAD_LAUNCH_CHECK();
+      hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)tiles), dim3(512), 0, s, d, tiles, counts, a);
+      TAD_LAUNCH_CHECK();
+      d.in = a;
+      u64* t = a; a = b; b = t;
+    }
+    a = b;
   }
 #define SUM_(T, V) launch_sum<T, V>(g, n, D, vocab, scale, accumulate, a, dout, ld_dout, dtable, ld_dtable, part, s)
   if (dout_dtype == TAD_BF16) {
@@ -379,9 +527,14 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
 #undef SUM_
   TAD_LAUNCH_CHECK();
   if (g.nchunks > 1) {
-    const int ct = (int)cdiv64(D, 64);
-    hipLaunchKernelGGL(embed_grad_join_kernel, dim3((unsigned)(g.nchunks * ct)), dim3(256), 0, s, n, D, vocab, g.S, ct, scale, accumulate, a, part,
-                       dtable, ld_dtable);
+    const int64_t most = g.nchunks - 1;
+    const int ct = (int)cdiv64(D, wide ? 256 : 64);
+    if (wide)
+      hipLaunchKernelGGL((embed_grad_join_kernel<4>), dim3((unsigned)(most * ct)), dim3(256), 0, s, n, D, vocab, g.S * GW, g.nchunks, ct, scale, accumulate,
+                         a, part, dtable, ld_dtable);
+    else
+      hipLaunchKernelGGL((embed_grad_join_kernel<1>), dim3((unsigned)(most * ct)), dim3(256), 0, s, n, D, vocab, g.S * GW, g.nchunks, ct, scale, accumulate,
+                         a, part, dtable, ld_dtable);
     TAD_LAUNCH_CHECK();
   }
   tad_note_kernel("embed_grad_sum_kernel");
