@@ -175,11 +175,15 @@ __global__ __launch_bounds__(512) void sort_move_kernel(Digit d, int tiles, cons
   for (int i = w0 + lane; i < w1; i += 64) atomicAdd(&at[wave][d.of(d.key(base + i))], 1u);
   // this thread's digit: how many in all tiles, in the tiles before
   uint32_t all = 0, before = 0;
-#pragma unroll 8
-  for (int t = 0; t < tiles; ++t) {
-    const uint32_t c = counts[t * MAX_BINS + tid];
-    all += c;
-    before += t < (int)blockIdx.x ? c : 0;
+  for (int t0 = 0; t0 < tiles; t0 += 32) {
+    uint32_t c[32];
+#pragma unroll
+    for (int t = 0; t < 32; ++t) c[t] = counts[(t0 + t < tiles ? t0 + t : 0) * MAX_BINS + tid];
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+      all += t0 + t < tiles ? c[t] : 0;
+      before += t0 + t < (int)blockIdx.x ? c[t] : 0;
+    }
   }
   uint32_t inc = all;
   for (int o = 1; o < 64; o <<= 1) {
@@ -198,20 +202,30 @@ __global__ __launch_bounds__(512) void sort_move_kernel(Digit d, int tiles, cons
   }
   __syncthreads();
   volatile uint32_t* mine = at[wave];        // this wave's alone from here on
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const bool on = i0 + lane < w1;
-    const u64 key = on ? d.key(base + i0 + lane) : 0;
-    const int g = d.of(key);
-    u64 same = __ballot(on);
-    for (int b = 1; b < d.bins; b <<= 1) {
-      const u64 set = __ballot(g & b);
-      same &= (g & b) ? set : ~set;
+  constexpr int U = 4;                       // keys of 64 lanes in flight
+  for (int i0 = w0; i0 < w1; i0 += 64 * U) {
+    u64 key[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + 64 * k + lane;
+      key[k] = d.key(base + (i < w1 ? i : w0));
     }
-    const int ahead = __popcll(same & ((1ull << lane) - 1));
-    if (on) {
-      const uint32_t p = mine[g];
-      out[p + ahead] = key;
-      if (ahead == 0) mine[g] = p + __popcll(same);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const bool on = i0 + 64 * k + lane < w1;
+      const int g = d.of(key[k]);
+      u64 same = __ballot(on);
+      if (same == 0) break;
+      for (int b = 1; b < d.bins; b <<= 1) {
+        const u64 set = __ballot(g & b);
+        same &= (g & b) ? set : ~set;
+      }
+      const int ahead = __popcll(same & ((1ull << lane) - 1));
+      if (on) {
+        const uint32_t p = mine[g];
+        out[p + ahead] = key[k];
+        if (ahead == 0) mine[g] = p + __popcll(same);
+      }
     }
   }
 }
@@ -503,7 +517,7 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
     hipLaunchKernelGGL(sort_rank_kernel, dim3((unsigned)cdiv64(n, 64)), dim3(1024), 0, s, (int)n, vocab, tokens, tok_stride, a);
     TAD_LAUNCH_CHECK();
   } else {
-    int bits = 1, tile = 2048;
+    int bits = 1, tile = 512;
     while (vocab >> bits) ++bits;                      // tokens 0 .. vocab (padding)
     while (cdiv64(n, tile) > MAX_TILES) tile *= 2;
     const int digits = (bits + 8) / 9, width = (bits + digits - 1) / digits, tiles = (int)cdiv64(n, tile);
