@@ -14,7 +14,7 @@
 #include <limits.h>
 #include <math.h>
 
-#include "common.h"
+#include "row_pieces.h"
 
 namespace {
 
@@ -175,33 +175,6 @@ __global__ __launch_bounds__(64) void sample_short_kernel(int64_t rows, int V, i
 }
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
-// A row as 16-byte pieces on the aligned grid: piece i holds the elements VEC i - a + (0 .. VEC - 1), a the row's distance
-// from the grid; the first and the last may be partly outside the row (-inf there, not loaded).
-template <typename T>
-struct Row {
-  static constexpr int VEC = 16 / sizeof(T);
-  typedef __attribute__((ext_vector_type(VEC))) T pack;
-  const T* x;
-  int64_t V, np;
-  int a;
-  __device__ Row(const T* x_, int64_t V_) : x(x_), V(V_) {
-    a = (int)(((uintptr_t)x_ / sizeof(T)) & (VEC - 1));
-    np = (V + a + VEC - 1) / VEC;
-  }
-  __device__ __forceinline__ int64_t first(int64_t i) const { return i * VEC - a; }
-  __device__ __forceinline__ void load(int64_t i, float (&v)[VEC]) const {
-    const int64_t j = first(i);
-    if (j >= 0 && j + VEC <= V) {
-      const pack p = *reinterpret_cast<const pack*>(x + j);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = (float)p[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = j + e >= 0 && j + e < V ? (float)x[j + e] : -INFINITY;
-    }
-  }
-};
-
 constexpr int BINS = 768;       // of log2 w, sixteen to the octave, down to 2^-48
 
 template <int NT>
@@ -273,11 +246,11 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V, const T* __restrict__ logits, int64_t ld, Settings st, int F,
                                                         const float* __restrict__ u, int64_t* __restrict__ out) {
   typedef RowState<NT> State;
-  constexpr int VEC = Row<T>::VEC, NW = State::NW, CAP = State::CAP;
+  constexpr int VEC = RowPieces<T>::VEC, NW = State::NW, CAP = State::CAP;
   __shared__ State S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
-  const Row<T> row(logits + r * ld, V);
+  const RowPieces<T> row(logits + r * ld, V);
   const RowSettings rs(st, r);
   // a wave's own contiguous share of the pieces
   const int64_t seg = (row.np + NW - 1) / NW, lo = wave * seg < row.np ? wave * seg : row.np, hi = lo + seg < row.np ? lo + seg : row.np;
