@@ -117,34 +117,31 @@ __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* log
 // ---------------------------------------------------------------- long rows: a workgroup per row
 // Two passes over the row: maximum and sum in one (every thread rescales its sum when its maximum grows), then the gradient,
 // from the row's end backwards, where the caches still hold it.
-template <int NW>
-__device__ __forceinline__ float block_sum(float v, float* s) {
-  v = wave_sum(v);
+template <int NW, bool MAX>
+__device__ __forceinline__ void block_two(float& a, float& b, float (*s)[NW]) {      // largest, or sum, of two values at once
+  a = MAX ? group_max<64>(a) : wave_sum(a);
+  b = MAX ? group_max<64>(b) : wave_sum(b);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) {
+    s[0][threadIdx.x >> 6] = a;
+    s[1][threadIdx.x >> 6] = b;
+  }
   __syncthreads();
-  float t = 0.f;
+  a = s[0][0];
+  b = s[1][0];
 #pragma unroll
-  for (int w = 0; w < NW; ++w) t += s[w];
-  return t;
-}
-template <int NW>
-__device__ __forceinline__ float block_max(float v, float* s) {
-  v = group_max<64>(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = s[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) t = fmaxf(t, s[w]);
-  return t;
+  for (int w = 1; w < NW; ++w) {
+    a = MAX ? fmaxf(a, s[0][w]) : a + s[0][w];
+    b = MAX ? fmaxf(b, s[1][w]) : b + s[1][w];
+  }
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_row_kernel(Args A, const T* logits, T* dlogits) {
+template <typename T, int NT, int H>
+__global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args A, const T* logits, T* dlogits) {
   constexpr int VEC = RowPieces<T>::VEC, NW = NT / 64;
   typedef typename RowPieces<T>::pack pack;
-  __shared__ float red[NW];
+  constexpr int KE = MAX_K / NT;                // the teacher's entries of a thread
+  __shared__ float red[2][NW];
   __shared__ float q[MAX_K];
   __shared__ int at[MAX_K];
   const int tid = threadIdx.x, K = A.K;
@@ -153,108 +150,124 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(Args A, const T* logits
   T* d = dlogits ? dlogits + r * A.ldd : nullptr;
   const RowPieces<T> row(x, V);
   const float w = A.weight ? A.weight[r] : 1.f;
-  float m = LOWEST, z = 0.f;
-  if (w != 0.f) {
-#pragma unroll 4
-    for (int64_t i = tid; i < row.np; i += NT) {
-      float v[VEC];
-      row.load(i, v);
-      float b = m;
+  float m = LOWEST, z = 0.f, tm = LOWEST, tz = 0.f;
+  // the entries and the student's logits at them, asked for before anything waits
+  int mine[KE];
+  float val[KE], xv[KE];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) b = fmaxf(b, v[e]);
-      float s = z * ex2((m - b) * A.c);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s += ex2((v[e] - b) * A.c);
-      m = b;
-      z = s;
-    }
-  }
-  const float mine = m;
-  m = block_max<NW>(m, red);
-  z = block_sum<NW>(z * ex2((mine - m) * A.c), red);
-  float tz = 0.f, tm = LOWEST;
-  if (w != 0.f && z != 0.f) {
-    for (int k = tid; k < K; k += NT) {
+  for (int n = 0; n < KE; ++n) {
+    const int k = tid + n * NT;
+    mine[n] = -1;
+    val[n] = xv[n] = 0.f;
+    if (k < K) {
       const int64_t i = A.index[r * A.ld_t + k];
-      at[k] = (uint64_t)i < (uint64_t)V ? (int)i : -1;
-      if (at[k] >= 0) tm = fmaxf(tm, A.value[r * A.ld_t + k]);
+      mine[n] = (uint64_t)i < (uint64_t)V ? (int)i : -1;
+      val[n] = A.value[r * A.ld_t + k];
+      if (mine[n] >= 0) xv[n] = (float)x[mine[n]];
     }
-    tm = block_max<NW>(tm, red);
-    for (int k = tid; k < K; k += NT) {
-      q[k] = at[k] >= 0 ? ex2((A.value[r * A.ld_t + k] - tm) * A.c) : 0.f;
-      tz += q[k];
-    }
-    tz = block_sum<NW>(tz, red);
   }
-  if (tz == 0.f) {          // the row counts nothing: weight 0, no student logit or no entry above -inf
+  const auto add = [&](const pack& p) {
+    float b = m;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) b = fmaxf(b, (float)p[e]);
+    float s = z * ex2((m - b) * A.c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s += ex2(((float)p[e] - b) * A.c);
+    m = b;
+    z = s;
+  };
+  pack held[H];
+  if (w != 0.f) {
+#pragma unroll
+    for (int k = 0; k < H; ++k)
+      if (tid + k * NT < row.np) held[k] = row.raw(tid + k * NT);
+#pragma unroll
+    for (int k = 0; k < H; ++k)
+      if (tid + k * NT < row.np) add(held[k]);
+#pragma unroll 4
+    for (int64_t i = tid + H * NT; i < row.np; i += NT) add(row.raw(i));
+  }
+#pragma unroll
+  for (int n = 0; n < KE; ++n)
+    if (mine[n] >= 0) tm = fmaxf(tm, val[n]);
+  const float own = m;
+  block_two<NW, true>(m, tm, red);
+  z *= ex2((own - m) * A.c);
+  float p[KE], qn[KE];
+#pragma unroll
+  for (int n = 0; n < KE; ++n) {
+    qn[n] = mine[n] >= 0 ? ex2((val[n] - tm) * A.c) : 0.f;
+    tz += qn[n];
+  }
+  block_two<NW, false>(z, tz, red);
+  if (w == 0.f || z == 0.f || tz == 0.f) {          // the row counts nothing
     if (tid == 0) A.loss[r] = 0.f;
     if (d)
       for (int64_t j = tid; j < V; j += NT) d[j] = (T)0.f;
     return;
   }
   const float itz = 1.f / tz, iz = 1.f / z, l2 = __log2f(tz) - __log2f(z), g = A.grad_scale * w * A.tau;
-  float l = 0.f;
-  float px[MAX_K / NT > 0 ? MAX_K / NT : 1];             // the student's p at this thread's entries, before the row may be overwritten
+  float l = 0.f, unused = 0.f;
 #pragma unroll
-  for (int n = 0; n < (MAX_K / NT > 0 ? MAX_K / NT : 1); ++n) {
-    const int k = tid + n * NT;
-    px[n] = 0.f;
-    if (k >= K) continue;
-    q[k] *= itz;
-    if (at[k] < 0) continue;
-    const float b = ((float)x[at[k]] - m) * A.c;
-    px[n] = ex2(b) * iz;
-    if (q[k] > 0.f) l += q[k] * ((A.value[r * A.ld_t + k] - tm) * A.c - b - l2);
+  for (int n = 0; n < KE; ++n) {
+    const float b = (xv[n] - m) * A.c;
+    p[n] = ex2(b) * iz;
+    qn[n] *= itz;
+    if (qn[n] > 0.f) l += qn[n] * ((val[n] - tm) * A.c - b - l2);
+    if (tid + n * NT < K) {
+      q[tid + n * NT] = qn[n];
+      at[tid + n * NT] = mine[n];
+    }
   }
-  l = block_sum<NW>(l, red);
+  block_two<NW, false>(l, unused, red);
   if (tid == 0) A.loss[r] = w * A.tau * A.tau * (l * LN2);
   if (!d) return;
-  __syncthreads();
   const float gz = g * iz;
   const bool together = (((uintptr_t)d ^ (uintptr_t)x) & 15) == 0;
-  const int64_t last = tid < row.np ? (row.np - 1 - tid) / NT * NT + tid : -1;
-#pragma unroll 4
-  for (int64_t i = last; i >= 0; i -= NT) {
-    float v[VEC];
-    row.load(i, v);
+  const auto put = [&](int64_t i, const pack& p) {
     pack o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = (T)(gz * ex2((v[e] - m) * A.c));
+    for (int e = 0; e < VEC; ++e) o[e] = (T)(gz * ex2(((float)p[e] - m) * A.c));
     const int64_t j = row.first(i);
     if (together && j >= 0 && j + VEC <= V) {
-      *reinterpret_cast<pack*>(d + j) = o;
+      __builtin_nontemporal_store(o, reinterpret_cast<pack*>(d + j));
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
         if (j + e >= 0 && j + e < V) d[j + e] = o[e];
     }
-  }
+  };
+#pragma unroll 4
+  for (int64_t i = tid < row.np ? (row.np - 1 - tid) / NT * NT + tid : -1; i >= H * NT; i -= NT) put(i, row.raw(i));
+#pragma unroll
+  for (int k = 0; k < H; ++k)
+    if (tid + k * NT < row.np) put(tid + k * NT, held[k]);
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < (MAX_K / NT > 0 ? MAX_K / NT : 1); ++n) {
-    const int k = tid + n * NT;
-    if (k >= K || at[k] < 0) continue;
-    float s = 0.f;
+  for (int n = 0; n < KE; ++n) {
+    if (mine[n] < 0) continue;
+    float sum = 0.f;
     bool first = true;
     for (int o = 0; o < K; ++o) {
-      if (at[o] != at[k]) continue;
-      if (o < k) first = false;
-      s += q[o];
+      if (at[o] != mine[n]) continue;
+      if (o < tid + n * NT) first = false;
+      sum += q[o];
     }
-    if (first) d[at[k]] = (T)(g * (px[n] - s));
+    if (first) d[mine[n]] = (T)(g * (p[n] - sum));
   }
 }
 
 template <typename T>
 int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
 #define SHORT_(G, E) hipLaunchKernelGGL((distill_short_kernel<T, G, E>), dim3((unsigned)cdiv64(A.rows, 256 / G)), dim3(256), 0, s, A, x, d)
-#define ROW_(NT) hipLaunchKernelGGL((distill_row_kernel<T, NT>), dim3((unsigned)A.rows), dim3(NT), 0, s, A, x, d)
+#define ROW_(NT, H) hipLaunchKernelGGL((distill_row_kernel<T, NT, H>), dim3((unsigned)A.rows), dim3(NT), 0, s, A, x, d)
   if (A.V <= 32) SHORT_(8, 4);
   else if (A.V <= 64) SHORT_(16, 4);
   else if (A.V <= 128) SHORT_(16, 8);
   else if (A.V <= 1024) SHORT_(64, 16);
-  else if (A.V <= 16384) ROW_(256);
-  else ROW_(1024);
+  else if (A.V <= 16384) ROW_(256, 4);
+  else if (A.V <= (sizeof(T) == 2 ? 65536 : 16384)) ROW_(512, 8);
+  else ROW_(512, 20);
 #undef SHORT_
 #undef ROW_
   TAD_LAUNCH_CHECK();

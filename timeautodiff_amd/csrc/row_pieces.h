@@ -16,15 +16,20 @@ struct RowPieces {
     np = (V + a + VEC - 1) / VEC;
   }
   __device__ __forceinline__ int64_t first(int64_t i) const { return i * VEC - a; }
-  __device__ __forceinline__ void load(int64_t i, float (&v)[VEC]) const {
+  __device__ __forceinline__ pack raw(int64_t i) const {
     const int64_t j = first(i);
+    pack p;
     if (j >= 0 && j + VEC <= V) {
-      const pack p = *reinterpret_cast<const pack*>(x + j);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = (float)p[e];
+      p = *reinterpret_cast<const pack*>(x + j);
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = j + e >= 0 && j + e < V ? (float)x[j + e] : -INFINITY;
+      for (int e = 0; e < VEC; ++e) p[e] = j + e >= 0 && j + e < V ? x[j + e] : (T)-INFINITY;
     }
+    return p;
+  }
+  __device__ __forceinline__ void load(int64_t i, float (&v)[VEC]) const {
+    const pack p = raw(i);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (float)p[e];
   }
 };
