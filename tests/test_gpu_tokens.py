@@ -303,10 +303,10 @@ SETTINGS = [(1.0, 0, 1.0, 0.0), (0.8, 50, 0.95, 0.02), (1.3, 0, 0.9, 0.0), (1.0,
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [1, 2, 5, 16, 17, 48, 64, 65, 100, 128, 129, 500, 1000, 1025, 4099, 20000, 32000])
+@pytest.mark.parametrize("V", [1, 2, 5, 16, 17, 48, 64, 65, 100, 128, 129, 256, 257, 500, 1000, 1024, 1025, 2048, 2049, 4099, 16384, 16385, 20000, 32000])
 def test_sample_tokens(ops, dev, dtype, V):
     rng = np.random.default_rng(V)
-    rows = 40 if V <= 1025 else 6
+    rows = 40 if V <= 2048 else 6
     for i, s in enumerate(SETTINGS):
         extra, offset = ((0, 0), (8, 0), (5, 1))[i % 3]
         logits, _ = strided(rows, V, extra, dtype, dev, offset=offset)

@@ -89,89 +89,177 @@ __device__ __forceinline__ u64 target_of(float u, u64 all) {
   return t < all ? t : all - 1;
 }
 
-// ---------------------------------------------------------------- rows of at most 64 logits: a thread per row
-// A wave lays 64 rows down in LDS, column by column, and every lane walks its own: V steps a pass, nothing exchanged
-// between lanes.  The cut is found by taking the next largest until enough are kept.
-constexpr int SHORT_V = 64;
+// ---------------------------------------------------------------- rows of up to 2048 logits: G lanes of a wave per row
+// The row and its weights stay in registers, a contiguous piece of E logits or fewer a lane; what the lanes share goes
+// across with DPP moves.  A cut is searched for by bisection: on the logits' values (their weights are exponential in them,
+// so a few steps separate neighbours), then, where a value does not lie between its neighbours any more, on the ordered
+// keys, so that it ends after at most 48 steps whatever the logits are.
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp(V v) {
+  if constexpr (sizeof(V) == 8) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+  } else {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+  }
+}
+template <typename V>
+__device__ __forceinline__ V lane_value(V v, int l) {
+  if constexpr (sizeof(V) == 8) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(V, (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l) << 32 |
+                                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l));
+  } else {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+  }
+}
+struct Add {
+  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Max {
+  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
+};
+struct Min {
+  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a < b ? a : b; }
+};
+template <int G, typename Op, typename V>
+__device__ __forceinline__ V across(V v) {
+  const Op op;
+  v = op(v, dpp<0xB1>(v));                    // quad_perm [1,0,3,2]
+  v = op(v, dpp<0x4E>(v));                    // quad_perm [2,3,0,1]
+  if constexpr (G >= 16) {
+    v = op(v, dpp<0x141>(v));                 // row_half_mirror
+    v = op(v, dpp<0x140>(v));                 // row_mirror
+  }
+  if constexpr (G == 64) v = op(op(lane_value(v, 0), lane_value(v, 16)), op(lane_value(v, 32), lane_value(v, 48)));
+  return v;
+}
+// what the lanes before this one hold together
+template <int G, typename V>
+__device__ __forceinline__ V lanes_before(V v, int lane) {
+  V inc = v;
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) {
+    const V up = __shfl_up(inc, o, G);
+    if (lane >= o) inc += up;
+  }
+  return inc - v;
+}
 
-template <typename T>
-__global__ __launch_bounds__(64) void sample_short_kernel(int64_t rows, int V, int lg, const T* __restrict__ logits, int64_t ld, Settings st, int F,
-                                                          const float* __restrict__ u, int64_t* __restrict__ out) {
-  extern __shared__ float s[];          // [V][65]
-  const int lane = threadIdx.x;
-  const int64_t r0 = (int64_t)blockIdx.x * 64;
-  const int sub = lane >> lg, c = lane & ((1 << lg) - 1), step = 64 >> lg;
-#pragma unroll 8
-  for (int i = sub; i < 64; i += step)
-    if (c < V) s[c * 65 + i] = r0 + i < rows ? (float)logits[(r0 + i) * ld + c] : -INFINITY;
-  __syncthreads();
-  const int64_t r = r0 + lane;
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, int per, const T* __restrict__ logits, int64_t ld, Settings st, int F,
+                                                           const float* __restrict__ u, int64_t* __restrict__ out) {
+  const int lane = threadIdx.x & (G - 1), j0 = lane * per;
+  const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (r >= rows) return;
-  const float* x = s + lane;
+  const T* x = logits + r * ld;
+#define EACH(...)                        \
+  _Pragma("unroll") for (int e = 0; e < E; ++e) { \
+    if (e >= per) break;                 \
+    __VA_ARGS__                          \
+  }
+  float v[E];
+  EACH(v[e] = j0 + e < V ? (float)x[j0 + e] : -INFINITY;)
   const RowSettings rs(st, r);
   float m = -INFINITY;
-  int first = -1;
-#pragma unroll 8
-  for (int v = 0; v < V; ++v) {
-    const float l = x[v * 65];
-    if (l > m) { m = l; first = v; }
-  }
-  if (first < 0 || !(rs.T > 0.0)) {
-    out[r] = first;
+  EACH(v[e] = v[e] > -INFINITY ? v[e] : -INFINITY; m = fmaxf(m, v[e]);)
+  m = across<G, Max>(m);
+  if (m == -INFINITY || !(rs.T > 0.0)) {
+    int at = V;
+    EACH(at = v[e] == m && e < at - j0 ? j0 + e : at;)
+    at = across<G, Min>(at);
+    if (lane == 0) out[r] = m == -INFINITY ? -1 : at;
     return;
   }
   const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
   const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
-  float cut = -INFINITY;                // kept: above `cut`, or equal to it at an index of at most `last`
-  int last = INT_MAX;
-  u64 kept = 0, whole = 0;
-  if (!by_k) {
-#pragma unroll 4
-    for (int v = 0; v < V; ++v) {
-      const float l = x[v * 65];
-      const double t = log2_weight(sc, l);
-      const u64 w = l > -INFINITY ? fixed_weight(sc, t) : 0;
-      whole += w;
-      kept += t >= rs.tmin ? w : 0;
+  u64 w[E];
+  uint32_t low = 0;                           // the ones below min_p
+  EACH(const double t = log2_weight(sc, v[e]); w[e] = v[e] > -INFINITY ? fixed_weight(sc, t) : 0ull; low |= t >= rs.tmin ? 0u : 1u << e;)
+
+  // halves the distance between two keys: by value as long as that lies between them
+  const auto between = [](uint32_t lo, uint32_t hi, int step) {
+    const uint32_t b = key_of(0.5f * logit_of(lo) + 0.5f * logit_of(hi));
+    return step < 16 && b > lo && b <= hi ? b : lo + (hi - lo + 1) / 2;
+  };
+  // drops what lies below `cut`, and of its equals (n of them) all but the first `ties`
+  const auto drop = [&](float cut, uint32_t ties, uint32_t n) {
+    uint32_t rank = 0;
+    if (ties < n) {
+      uint32_t mine = 0;
+      EACH(mine += v[e] == cut;)
+      rank = lanes_before<G>(mine, lane);
     }
-  }
-  for (int pass = by_k ? 0 : 1; pass < (by_p ? 2 : 1); ++pass) {
-    const u64 need = pass == 1 ? mass_needed(rs.p, whole) : ~0ull;
-    const int most = by_k ? (int)rs.k : V;
-    u64 mass = 0;
-    kept = 0;
-    cut = INFINITY;
-    last = -1;
-    for (int n = 0; n < most && mass < need; ++n) {
-      float b = -INFINITY;
-      int at = -1;
-#pragma unroll 8
-      for (int v = 0; v < V; ++v) {
-        const float l = x[v * 65];
-        if ((l < cut || (l == cut && v > last)) && l > b) { b = l; at = v; }
+    EACH(const bool gone = v[e] < cut || (ties < n && v[e] == cut && rank++ >= ties); v[e] = gone ? -INFINITY : v[e]; w[e] = gone ? 0 : w[e];)
+  };
+
+  if (by_k) {
+    int n = 0;
+    uint32_t lo = UINT_MAX, hi = key_of(m);
+    EACH(n += v[e] > -INFINITY; const uint32_t k = key_of(v[e]); lo = k && k < lo ? k : lo;)
+    n = across<G, Add>(n);
+    lo = across<G, Min>(lo);
+    if (n > rs.k) {
+      const int want = (int)rs.k;
+      int c = n;                              // that many reach `lo`
+      for (int step = 0; lo < hi && c != want; ++step) {
+        const uint32_t b = between(lo, hi, step);
+        const float f = logit_of(b);
+        int k = 0;
+        EACH(k += v[e] >= f;)
+        k = across<G, Add>(k);
+        if (k >= want) { lo = b; c = k; } else hi = b - 1;
       }
-      if (at < 0) break;
-      cut = b;
-      last = at;
-      const double t = log2_weight(sc, b);
-      const u64 w = fixed_weight(sc, t);
-      mass += w;
-      if (t >= rs.tmin) kept += w;
-    }
-    whole = mass;
-  }
-  const u64 target = target_of(u[r], kept);
-  u64 run = 0;
-  for (int v = 0; v < V; ++v) {
-    const float l = x[v * 65];
-    if (!(l > cut || (l == cut && v <= last)) || !(l > -INFINITY)) continue;
-    const double t = log2_weight(sc, l);
-    if (t >= rs.tmin) run += fixed_weight(sc, t);
-    if (run > target) {
-      out[r] = v;
-      break;
+      const float cut = logit_of(lo);
+      uint32_t eq = 0;
+      EACH(eq += v[e] == cut;)
+      eq = across<G, Add>(eq);
+      drop(cut, eq - (uint32_t)(c - want), eq);
     }
   }
+  if (by_p) {
+    u64 whole = 0;
+    int n = 0;
+    uint32_t lo = UINT_MAX, hi = key_of(m);
+    EACH(whole += w[e]; n += w[e] != 0; const uint32_t k = key_of(v[e]); lo = w[e] && k < lo ? k : lo;)
+    whole = across<G, Add>(whole);
+    n = across<G, Add>(n);
+    lo = across<G, Min>(lo);
+    const u64 need = mass_needed(rs.p, whole);
+    int above = 0;                            // n reach `lo`, `above` lie above `hi`
+    for (int step = 0; lo < hi && n - above > 1; ++step) {
+      const uint32_t b = between(lo, hi, step);
+      const float f = logit_of(b);
+      u64 mass = 0;
+      int k = 0;
+      EACH(const bool in = v[e] >= f; mass += in ? w[e] : 0ull; k += in;)
+      mass = across<G, Add>(mass);
+      k = across<G, Add>(k);
+      if (mass >= need) { lo = b; n = k; } else { hi = b - 1; above = k; }
+    }
+    const float cut = logit_of(lo);
+    uint32_t eq = (uint32_t)(n - above), ties = eq;
+    if (eq > 1) {                             // (lo = hi: equals)
+      u64 mass = 0, one = 0;
+      EACH(mass += v[e] > cut ? w[e] : 0ull; one = v[e] == cut ? w[e] : one;)
+      mass = across<G, Add>(mass);
+      one = across<G, Max>(one);
+      ties = (uint32_t)((need - mass + one - 1) / one);
+    }
+    drop(cut, ties, eq);
+  }
+  u64 mine = 0;
+  EACH(w[e] = low >> e & 1 ? 0ull : w[e]; mine += w[e];)
+  const u64 all = across<G, Add>(mine), target = target_of(u[r], all);
+  u64 run = lanes_before<G>(mine, lane);
+  if (run <= target && target < run + mine) {
+    int at = 0;
+    EACH(run += w[e]; at += run <= target;)
+    out[r] = j0 + at;
+  }
+#undef EACH
 }
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
@@ -584,13 +672,20 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
 template <typename T>
 int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const Settings& st, int F, const float* u, int64_t* out, hipStream_t s) {
   const T* x = (const T*)logits;
-  if (V <= SHORT_V) {
-    int lg = 0;
-    while ((1 << lg) < V) ++lg;
-    hipLaunchKernelGGL(sample_short_kernel<T>, dim3((unsigned)cdiv64(rows, 64)), dim3(64), (size_t)V * 65 * 4, s, rows, (int)V, lg, x, ld, st, F, u,
-                       out);
+#define GROUP_(G, E)                                                                                                                             \
+  hipLaunchKernelGGL((sample_group_kernel<T, G, E>), dim3((unsigned)cdiv64(rows, 256 / G)), dim3(256), 0, s, rows, (int)V, (int)cdiv64(V, G), x, ld, \
+                     st, F, u, out)
+  if (V <= 16) {
+    GROUP_(4, 4);
+  } else if (V <= 64) {
+    GROUP_(4, 16);
+  } else if (V <= 256) {
+    GROUP_(16, 16);
+  } else if (V <= 1024) {
+    GROUP_(64, 16);
   } else if (V <= 2048) {
-    hipLaunchKernelGGL((sample_row_kernel<T, 64>), dim3((unsigned)rows), dim3(64), 0, s, rows, V, x, ld, st, F, u, out);
+    GROUP_(64, 32);
+#undef GROUP_
   } else if (V <= 16384) {
     hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, x, ld, st, F, u, out);
   } else {
