@@ -601,10 +601,11 @@ int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dty
  *   is at least top_p of theirs (1 or more: all; at least one is kept); of those the ones with w_j >= min_p (0: all);
  *   out[r] = the lowest index j at which the sum of the kept w up to j exceeds u[r] times the sum of all kept w.
  * Ties go to the lowest index.  T = 0 takes the largest logit.  -inf and NaN logits are never drawn; a row with no other
- * gives -1; among +inf logits the draw is even.  Each setting is one number, or, where its _rows pointer is given, a number
+ * gives -1; +inf counts as the largest float32 number.  Each setting is one number, or, where its _rows pointer is given, a number
  * per row (T, top_p, min_p float32, top_k int32; there T not above 0 means 0, top_k below 1 means all, min_p above 1 means 1;
  * NaN: T 0, the others off).  u below 0 or NaN counts as 0, u of 1 or more gives the last kept token.  The masses are
- * integers, multiples of 2^-44 of the largest weight (fewer bits from 2^18 logits on): every sum is exact. */
+ * whole multiples of 2^-F of the largest weight (F = 44; 62 - log2 V from 2^18 logits on, 53 - log2 V from 512 to 2048): every
+ * sum is exact. */
 int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, int dtype, int64_t ld, double temperature, const float* temperature_rows,
                       int64_t top_k, const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
                       const float* min_p_rows, const float* u, int64_t* out, tad_stream_t stream);

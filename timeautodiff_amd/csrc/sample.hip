@@ -4,10 +4,11 @@
 //   their mass; of those the ones with w_j >= min_p.  The answer is the lowest index at which the running sum of the kept
 //   w, by index, exceeds u times their sum.  Ties go to the lowest index.
 //
-// The answer is an index that a sum decides, so the sums are exact: every w is rounded once to a multiple of 2^-F (F = 44
-// for rows of up to 2^18 logits) and added as a 64-bit integer.  The order of additions then changes nothing, and the
-// answer is the real numbers' unless u lies within about 2^-40 of a border.  Float64 fused multiply-adds issue at the rate
-// of float32 ones here, so such a weight costs about 20 instructions.
+// The answer is an index that a sum decides, so the sums are exact: every w is rounded once to a whole multiple of 2^-F (F =
+// 44 for rows of up to 512 logits and of 2049 to 2^18, else a few less) and added as a whole number, in float64 where all
+// of a sum fits its 53 bits and in 64-bit integers beyond.  The order of additions then changes nothing, and the answer is the
+// real numbers' unless u lies within about 2^-40 of a border.  Float64 fused multiply-adds issue at the rate of float32 ones
+// here, so such a weight costs about 20 instructions.
 //
 // Every filter keeps a prefix of the row in falling order (ties by index), so their conjunction is the shortest of the
 // prefixes: one cut (a key, and how many of those that equal it).
@@ -35,31 +36,33 @@ struct Scale {
   double c;         // log2(e) / T
   int F;            // weights are multiples of 2^-F
 };
-// log2 of w
-__device__ __forceinline__ double log2_weight(const Scale& s, float l) { return l == s.m ? 0.0 : ((double)l - (double)s.m) * s.c; }
-// 2^t in units of 2^-F, rounded: 2^n times the series of e^z, z = ln 2 (t - n), |z| <= 0.347, whose first term left out is below
-// 2^-47; the last bits come out of the addition of 2^52
-__device__ __forceinline__ u64 fixed_weight(const Scale& s, double t) {
-  if (!(t > -48.0)) return 0;                       // (NaN: -inf / inf)
-  const double n = rint(t), z = (t - n) * 0.6931471805599453094;
-  double p = 1.0 / 479001600;
-  p = __builtin_fma(p, z, 1.0 / 39916800);
-  p = __builtin_fma(p, z, 1.0 / 3628800);
-  p = __builtin_fma(p, z, 1.0 / 362880);
-  p = __builtin_fma(p, z, 1.0 / 40320);
-  p = __builtin_fma(p, z, 1.0 / 5040);
-  p = __builtin_fma(p, z, 1.0 / 720);
-  p = __builtin_fma(p, z, 1.0 / 120);
-  p = __builtin_fma(p, z, 1.0 / 24);
-  p = __builtin_fma(p, z, 1.0 / 6);
-  p = __builtin_fma(p, z, 0.5);
-  p = __builtin_fma(p, z, 1.0);
-  p = __builtin_fma(p, z, 1.0);
-  return __builtin_bit_cast(u64, __builtin_amdgcn_ldexp(p, (int)n + s.F) + 4503599627370496.0) & 0xfffffffffffffull;
+// log2 of w; NaN logits, and -inf whatever T is, count as 2^-100
+__device__ __forceinline__ double log2_weight(const Scale& s, float l) { return fmax(((double)l - (double)s.m) * s.c, -100.0); }
+// 2^t in units of 2^-F, rounded to a whole number (0 from about t = -F - 1 down): 2^n times the series of 2^f = e^(f ln 2),
+// |f| <= 1/2, whose first term left out is below 2^-52
+__device__ __forceinline__ double fixed_weight(const Scale& s, double t) {
+  constexpr double L = 0.6931471805599453094;
+  constexpr double L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L4 * L2, L7 = L6 * L, L8 = L4 * L4, L9 = L8 * L, L10 = L8 * L2, L11 = L10 * L,
+                   L12 = L8 * L4;
+  const double n = rint(t), f = t - n;
+  double p = L12 / 479001600;
+  p = __builtin_fma(p, f, L11 / 39916800);
+  p = __builtin_fma(p, f, L10 / 3628800);
+  p = __builtin_fma(p, f, L9 / 362880);
+  p = __builtin_fma(p, f, L8 / 40320);
+  p = __builtin_fma(p, f, L7 / 5040);
+  p = __builtin_fma(p, f, L6 / 720);
+  p = __builtin_fma(p, f, L5 / 120);
+  p = __builtin_fma(p, f, L4 / 24);
+  p = __builtin_fma(p, f, L3 / 6);
+  p = __builtin_fma(p, f, L2 / 2);
+  p = __builtin_fma(p, f, L);
+  p = __builtin_fma(p, f, 1.0);
+  return rint(__builtin_amdgcn_ldexp(p, (int)n + s.F));
 }
-__device__ __forceinline__ u64 weight_of(const Scale& s, float l) {
-  return l > -INFINITY ? fixed_weight(s, log2_weight(s, l)) : 0ull;
-}
+__device__ __forceinline__ double weight_of(const Scale& s, float l) { return fixed_weight(s, log2_weight(s, l)); }
+// sum + w where `in`: one move and one multiply-add
+__device__ __forceinline__ double add_if(bool in, double w, double sum) { return __builtin_fma(in ? 1.0 : 0.0, w, sum); }
 
 struct Settings {
   double T, p, minp;
@@ -78,16 +81,23 @@ struct RowSettings {
     tmin = m > 0.0 ? log2(m < 1.0 ? m : 1.0) : -INFINITY;
   }
 };
-// the mass that a prefix has to reach, and the sum that has to be exceeded
+// all in units of 2^-F: the mass that a prefix has to reach; how many weights `one` reach what is left of it; the sum that
+// has to be exceeded
 __device__ __forceinline__ u64 mass_needed(double p, u64 whole) {
   const double d = ceil((p > 0.0 ? p : 0.0) * (double)whole);
   const u64 n = d >= 1.0 ? (u64)d : 1;
   return n < whole ? n : whole;
 }
+__device__ __forceinline__ double mass_needed(double p, double whole) { return fmin(fmax(ceil(p * whole), 1.0), whole); }
+__device__ __forceinline__ u64 ties_needed(u64 left, u64 one) { return one ? (left + one - 1) / one : 1; }
+__device__ __forceinline__ u64 ties_needed(double left, double one) { return ties_needed((u64)left, (u64)one); }
 __device__ __forceinline__ u64 target_of(float u, u64 all) {
   const u64 t = u > 0.f ? (u >= 1.f ? all : (u64)((double)u * (double)all)) : 0;
   return t < all ? t : all - 1;
 }
+__device__ __forceinline__ double target_of(float u, double all) { return fmin(floor((u > 0.f ? (double)u : 0.0) * all), all - 1.0); }
+
+constexpr float LARGEST = 3.4028234663852886e38f;      // what +inf counts as
 
 // ---------------------------------------------------------------- rows of up to 2048 logits: G lanes of a wave per row
 // The row and its weights stay in registers, a contiguous piece of E logits or fewer a lane; what the lanes share goes
@@ -157,14 +167,13 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
   const T* x = logits + r * ld;
 #define EACH(...)                        \
   _Pragma("unroll") for (int e = 0; e < E; ++e) { \
-    if (e >= per) break;                 \
     __VA_ARGS__                          \
   }
   float v[E];
-  EACH(v[e] = j0 + e < V ? (float)x[j0 + e] : -INFINITY;)
+  EACH(v[e] = e < per && j0 + e < V ? (float)x[j0 + e] : -INFINITY;)
   const RowSettings rs(st, r);
   float m = -INFINITY;
-  EACH(v[e] = v[e] > -INFINITY ? v[e] : -INFINITY; m = fmaxf(m, v[e]);)
+  EACH(v[e] = v[e] > -INFINITY ? fminf(v[e], LARGEST) : -INFINITY; m = fmaxf(m, v[e]);)
   m = across<G, Max>(m);
   if (m == -INFINITY || !(rs.T > 0.0)) {
     int at = V;
@@ -175,9 +184,9 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
   }
   const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
   const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
-  u64 w[E];
+  double w[E];
   uint32_t low = 0;                           // the ones below min_p
-  EACH(const double t = log2_weight(sc, v[e]); w[e] = v[e] > -INFINITY ? fixed_weight(sc, t) : 0ull; low |= t >= rs.tmin ? 0u : 1u << e;)
+  EACH(const double t = log2_weight(sc, v[e]); w[e] = fixed_weight(sc, t); low |= t >= rs.tmin ? 0u : 1u << e;)
 
   // halves the distance between two keys: by value as long as that lies between them
   const auto between = [](uint32_t lo, uint32_t hi, int step) {
@@ -220,21 +229,21 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
     }
   }
   if (by_p) {
-    u64 whole = 0;
+    double whole = 0;
     int n = 0;
     uint32_t lo = UINT_MAX, hi = key_of(m);
-    EACH(whole += w[e]; n += w[e] != 0; const uint32_t k = key_of(v[e]); lo = w[e] && k < lo ? k : lo;)
+    EACH(whole += w[e]; n += w[e] != 0; const uint32_t k = key_of(v[e]); lo = w[e] != 0 && k < lo ? k : lo;)
     whole = across<G, Add>(whole);
     n = across<G, Add>(n);
     lo = across<G, Min>(lo);
-    const u64 need = mass_needed(rs.p, whole);
+    const double need = mass_needed(rs.p, whole);
     int above = 0;                            // n reach `lo`, `above` lie above `hi`
     for (int step = 0; lo < hi && n - above > 1; ++step) {
       const uint32_t b = between(lo, hi, step);
       const float f = logit_of(b);
-      u64 mass = 0;
+      double mass = 0;
       int k = 0;
-      EACH(const bool in = v[e] >= f; mass += in ? w[e] : 0ull; k += in;)
+      EACH(const bool in = v[e] >= f; mass = add_if(in, w[e], mass); k += in;)
       mass = across<G, Add>(mass);
       k = across<G, Add>(k);
       if (mass >= need) { lo = b; n = k; } else { hi = b - 1; above = k; }
@@ -242,18 +251,18 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
     const float cut = logit_of(lo);
     uint32_t eq = (uint32_t)(n - above), ties = eq;
     if (eq > 1) {                             // (lo = hi: equals)
-      u64 mass = 0, one = 0;
-      EACH(mass += v[e] > cut ? w[e] : 0ull; one = v[e] == cut ? w[e] : one;)
+      double mass = 0, one = 0;
+      EACH(mass = add_if(v[e] > cut, w[e], mass); one = v[e] == cut ? w[e] : one;)
       mass = across<G, Add>(mass);
       one = across<G, Max>(one);
-      ties = (uint32_t)((need - mass + one - 1) / one);
+      ties = (uint32_t)ties_needed(need - mass, one);
     }
     drop(cut, ties, eq);
   }
-  u64 mine = 0;
-  EACH(w[e] = low >> e & 1 ? 0ull : w[e]; mine += w[e];)
-  const u64 all = across<G, Add>(mine), target = target_of(u[r], all);
-  u64 run = lanes_before<G>(mine, lane);
+  double mine = 0;
+  EACH(w[e] = low >> e & 1 ? 0.0 : w[e]; mine += w[e];)
+  const double all = across<G, Add>(mine), target = target_of(u[r], all);
+  double run = lanes_before<G>(mine, lane);
   if (run <= target && target < run + mine) {
     int at = 0;
     EACH(run += w[e]; at += run <= target;)
@@ -263,25 +272,32 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
 }
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
-constexpr int BINS = 768;       // of log2 w, sixteen to the octave, down to 2^-48
+constexpr int BINS = 1024, BINS_OCTAVE = 64;       // of log2 w, down to 2^-16
+constexpr int PAIRS = 256;                         // candidates that are compared each with each
 
+struct Candidate {
+  u64 k;             // key << 32 | ~index: falling logits, equal ones by index
+  double w;
+};
 template <int NT>
 struct RowState {
-  static constexpr int NW = NT / 64;
-  static constexpr int CAP = NT < 256 ? 256 : NT;       // candidates
+  static constexpr int NW = NT / 64, CAP = 1024;
   u64 list[CAP];
-  u64 mass[BINS];
-  uint32_t cnt[256];
+  union {
+    u64 mass[BINS];
+    Candidate pair[PAIRS];
+  };
   u64 wsum[NW];
   uint32_t wcnt[NW];
-  uint32_t n, key, n_above;
+  float wmax[NW], wmin[NW];
+  uint32_t n, key, ties;
   u64 above;
+  double total;
 };
 
 template <int NT, typename I>
 __device__ __forceinline__ I block_total(I v, I* s) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  if constexpr (NT == 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -340,87 +356,129 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   const int64_t r = blockIdx.x;
   const RowPieces<T> row(logits + r * ld, V);
   const RowSettings rs(st, r);
+  const float uu = u[r];
   // a wave's own contiguous share of the pieces
   const int64_t seg = (row.np + NW - 1) / NW, lo = wave * seg < row.np ? wave * seg : row.np, hi = lo + seg < row.np ? lo + seg : row.np;
+  bool infinite = false;                    // +inf among the logits
 
-#define EACH_PIECE(...)                                   \
-  _Pragma("unroll 4") for (int64_t i = lo + lane; i < hi; i += 64) { \
-    float v[VEC];                                         \
-    row.load(i, v);                                       \
-    __VA_ARGS__                                           \
+  // every piece of the share, and every element of the piece (v[e])
+#define EACH_PIECE(...) _Pragma("unroll 4") ONE_BY_ONE(__VA_ARGS__)
+#define ONE_BY_ONE(...)                                                                  \
+  for (int64_t i = lo + lane; i < hi; i += 64) {                                         \
+    float v[VEC];                                                                        \
+    row.load(i, v);                                                                      \
+    if (infinite) {                                                                      \
+      _Pragma("unroll") for (int e = 0; e < VEC; ++e) v[e] = v[e] == INFINITY ? LARGEST : v[e]; \
+    }                                                                                    \
+    __VA_ARGS__                                                                          \
   }
+#define EACH(...) _Pragma("unroll") for (int e = 0; e < VEC; ++e) { __VA_ARGS__ }
 
-  // the largest logit of the thread, then of the row
+  // the thread's largest logit, the row's, and the smallest of the threads'
   float tm = -INFINITY;
-  EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) tm = v[e] > tm ? v[e] : tm;)
-  float m = tm;
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if constexpr (NT > 64) {
-    float* f = reinterpret_cast<float*>(S.wcnt);
-    if (lane == 0) f[wave] = m;
-    __syncthreads();
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, f[w]);
-    __syncthreads();
+  EACH_PIECE(EACH(tm = fmaxf(tm, v[e]);))
+  float m = across<64, Max>(tm), least = across<64, Min>(tm > -INFINITY ? tm : INFINITY);
+  if (lane == 0) {
+    S.wmax[wave] = m;
+    S.wmin[wave] = least;
+  }
+  if (tid == 0) S.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    m = fmaxf(m, S.wmax[w]);
+    least = fminf(least, S.wmin[w]);
   }
   if (m == -INFINITY) {
     if (tid == 0) out[r] = -1;
     return;
   }
   if (!(rs.T > 0.0)) {
-    u64 at = ~0ull;                       // the lowest index of the largest
-    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) if (v[e] == m) {
-      const u64 j = (u64)(row.first(i) + e);
-      at = j < at ? j : at;
-    })
-    for (int o = 32; o > 0; o >>= 1) {
-      const u64 b = __shfl_xor(at, o);
-      at = b < at ? b : at;
-    }
+    u64 at = ~0ull;                         // the lowest index of the largest
+    EACH_PIECE(EACH(const u64 j = (u64)(row.first(i) + e); at = v[e] == m && j < at ? j : at;))
+    at = across<64, Min>(at);
     if (lane == 0) S.wsum[wave] = at;
     __syncthreads();
     for (int w = 0; w < NW; ++w) at = S.wsum[w] < at ? S.wsum[w] : at;
     if (tid == 0) out[r] = (int64_t)at;
     return;
   }
+  infinite = m == INFINITY;
+  m = fminf(m, LARGEST);
+  tm = fminf(tm, LARGEST);
   const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
   const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
+  // halves the distance between two keys: by value as long as that lies between them
+  const auto between = [](uint32_t a, uint32_t b, int step) {
+    const uint32_t k = key_of(0.5f * logit_of(a) + 0.5f * logit_of(b));
+    return step < 16 && k > a && k <= b ? k : a + (b - a + 1) / 2;
+  };
 
   // ---- few candidates: all that top-k can keep fits the list
-  if ((by_k && rs.k <= CAP / 2) || ((by_k || by_p) && V <= CAP)) {
+  if ((by_k && rs.k <= CAP / 2 && rs.k <= NT) || ((by_k || by_p) && V <= CAP)) {
     const int64_t kk = by_k ? rs.k : V;
-    uint32_t thr = 0;
-    if (V > CAP) {
-      // kk threads whose largest is at least `thr`: so at least kk logits are; 16 bits of it are enough (NT < kk: no thread's
-      // largest says anything, and the list runs over)
-      const uint32_t mine = key_of(tm);
-      for (int bit = 31; bit >= 16; --bit) {
-        const uint32_t t = thr | 1u << bit;
-        int n = __popcll(__ballot(mine >= t));
-        if constexpr (NT > 64) n = __syncthreads_count(mine >= t);
-        if (n >= kk) thr = t;
+    // where kk threads' largest reach `floor`, at least kk logits do; not many more than kk are wanted
+    float floor = -LARGEST;
+    if (V > CAP && __syncthreads_count(tm >= least) >= kk) {
+      uint32_t a = key_of(least), b = key_of(m);
+      for (int step = 0; step < 24 && a < b; ++step) {
+        const uint32_t k = between(a, b, step);
+        const int n = __syncthreads_count(tm >= logit_of(k));
+        if (n >= kk) a = k; else b = k - 1;
+        if (n >= kk && n <= kk + kk / 4 + 8) break;
       }
+      floor = logit_of(a);
     }
-    if (thr == 0) thr = 1;
-    if (tid == 0) S.n = 0;
+    EACH_PIECE(EACH(if (v[e] >= floor) {
+      const uint32_t at = atomicAdd(&S.n, 1u);
+      if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+    }))
     __syncthreads();
-    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
-      const uint32_t key = key_of(v[e]);
-      if (key >= thr) {
-        const uint32_t at = atomicAdd(&S.n, 1u);
-        if (at < CAP) S.list[at] = (u64)key << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+    const int n = S.n < CAP + 1 ? (int)S.n : CAP + 1, nk = kk < n ? (int)kk : n;
+    if (n <= PAIRS) {
+      // each with each: its place and the mass above it in falling order, then the kept mass below it by index
+      const bool on = tid < n;
+      const u64 mine = on ? S.list[tid] : 0;
+      const double t = on ? log2_weight(sc, logit_of((uint32_t)(mine >> 32))) : -100.0, w = fixed_weight(sc, t);
+      if (on) S.pair[tid] = {mine, w};
+      __syncthreads();
+      double above = 0;
+      int rank = 0;
+      if (on) {
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+          const Candidate c = S.pair[j];
+          const bool in = c.k > mine;
+          rank += in;
+          above = add_if(in, c.w, above);
+        }
+        if (rank == nk - 1) S.total = above + w;
       }
-    })
-    __syncthreads();
-    const uint32_t n = S.n;
+      __syncthreads();
+      const bool keep = on && rank < nk && (!by_p || above < mass_needed(rs.p, S.total)) && t >= rs.tmin;
+      if (on) S.pair[tid].w = keep ? w : 0.0;
+      __syncthreads();
+      if (!keep) return;
+      double before = 0, all = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const Candidate c = S.pair[j];
+        before = add_if((uint32_t)c.k > (uint32_t)mine, c.w, before);
+        all += c.w;
+      }
+      const double target = target_of(uu, all);
+      if (before <= target && target < before + w) out[r] = (int64_t)(uint32_t)~(uint32_t)mine;
+      return;
+    }
     if (n <= CAP) {
-      const int P = pow2_at_least((int)n);
+      // sorted: by logit for the cut, the kept ones by index for the answer
+      const int P = pow2_at_least(n);
       for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
       sort_list<NT>(S.list, P, true);
-      const int nk = kk < n ? (int)kk : (int)n;
       u64 whole = 0;
       if (by_p) {
         u64 w = 0;
-        for (int i = tid; i < nk; i += NT) w += weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)));
+        for (int i = tid; i < nk; i += NT) w += (u64)weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)));
         whole = block_total<NT>(w, S.wsum);
       }
       const u64 need = by_p ? mass_needed(rs.p, whole) : ~0ull;
@@ -428,8 +486,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       uint32_t nkept = 0;
       for (int base = 0; base < nk; base += NT) {
         const int i = base + tid;
-        const double t = i < nk ? log2_weight(sc, logit_of((uint32_t)(S.list[i] >> 32))) : -INFINITY;
-        const u64 w = i < nk ? fixed_weight(sc, t) : 0;
+        const double t = i < nk ? log2_weight(sc, logit_of((uint32_t)(S.list[i] >> 32))) : -100.0;
+        const u64 w = i < nk ? (u64)fixed_weight(sc, t) : 0;
         u64 sum;
         const u64 before = above + block_scan<NT>(w, S.wsum, &sum);
         const bool keep = i < nk && before < need && t >= rs.tmin;
@@ -437,7 +495,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
         kept += block_total<NT>(keep ? w : 0ull, S.wsum);
         above += sum;
       }
-      // by index: index << 32 | key, rising
+      // index << 32 | key, rising
       const int Q = pow2_at_least((int)nkept);
       __syncthreads();
       for (int i = tid; i < Q; i += NT) {
@@ -445,11 +503,11 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
         S.list[i] = i < (int)nkept ? (u64)(uint32_t)~(uint32_t)a << 32 | a >> 32 : ~0ull;
       }
       sort_list<NT>(S.list, Q, false);
-      const u64 target = target_of(u[r], kept);
+      const u64 target = target_of(uu, kept);
       u64 run = 0;
       for (int base = 0; base < (int)nkept; base += NT) {
         const int i = base + tid;
-        const u64 w = i < (int)nkept ? weight_of(sc, logit_of((uint32_t)S.list[i])) : 0;
+        const u64 w = i < (int)nkept ? (u64)weight_of(sc, logit_of((uint32_t)S.list[i])) : 0;
         u64 sum;
         const u64 before = run + block_scan<NT>(w, S.wsum, &sum);
         if (before <= target && target < before + w) out[r] = (int64_t)(S.list[i] >> 32);
@@ -458,215 +516,189 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       return;
     }
     __syncthreads();
+    if (tid == 0) S.n = 0;
   }
 
-  // ---- the cut: every key above `cut`, and the first `ties` (by index) that equal it (ALL: no need to count them)
+  // ---- the cut: every logit above `cut`, and the first `ties` (by index) that equal it (ALL: no need to count them)
   constexpr uint32_t ALL = UINT_MAX;
-  uint32_t cut = 0, ties = ALL;
-  u64 whole = 0, need = 0;                 // mass of what top-k keeps, and top_p of it
-  bool found = false;
-  if (by_p && !by_k) {
-    // masses by log2 w; the bin in which the sum from above reaches what is needed is looked at closely
-    for (int b = tid; b < BINS; b += NT) S.mass[b] = 0;
-    if (tid == 0) S.n = 0;
-    __syncthreads();
-    u64 sum = 0;
-    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
-      const double t = log2_weight(sc, v[e]);
-      if (v[e] > -INFINITY && t > -48.0) {
-        const u64 w = fixed_weight(sc, t);
-        sum += w;
-        atomicAdd(&S.mass[(int)(t * -16.0)], w);
+  float cut = -LARGEST;
+  uint32_t ties = ALL;
+  // how many logits reach f, and how many of them equal it; the mass of what reaches f (with top-k's ties, if f is its cut)
+  const auto count = [&](float f) {
+    uint32_t n = 0;
+    EACH_PIECE(EACH(n += v[e] >= f;))
+    return block_total<NT>(n, S.wcnt);
+  };
+  const auto mass_from = [&](float f) {
+    double w = 0;
+    ONE_BY_ONE(float b = -INFINITY; EACH(b = fmaxf(b, v[e]);) if (__any(b >= f)) EACH(w = add_if(v[e] >= f, weight_of(sc, v[e]), w);))
+    return block_total<NT>((u64)w, S.wsum);
+  };
+  const auto above_of = [](float f) { return logit_of(key_of(f) + 1); };      // the next larger value
+  if (by_k) {
+    const uint32_t n = count(-LARGEST);
+    if (n > rs.k) {
+      const uint32_t want = (uint32_t)rs.k;
+      uint32_t a = key_of(-LARGEST), b = key_of(m), c = n;
+      for (int step = 0; a < b && c != want; ++step) {
+        const uint32_t k = between(a, b, step), got = count(logit_of(k));
+        if (got >= want) { a = k; c = got; } else b = k - 1;
       }
-    })
-    whole = block_total<NT>(sum, S.wsum);
-    need = mass_needed(rs.p, whole);
-    __syncthreads();
-    u64 above = 0;
-    for (int base = 0; base < BINS; base += NT) {
-      const int b = base + tid;
-      const u64 w = b < BINS ? S.mass[b] : 0;
-      u64 all;
-      const u64 before = above + block_scan<NT>(w, S.wsum, &all);
-      if (before < need && need <= before + w) { S.key = (uint32_t)b; S.above = before; }
-      above += all;
+      cut = logit_of(a);
+      if (c != want) ties = want - (cut < m ? count(above_of(cut)) : 0);
     }
-    __syncthreads();
-    const int bin = (int)S.key;
-    above = S.above;
-    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
-      const double t = log2_weight(sc, v[e]);
-      if (v[e] > -INFINITY && t > -48.0 && (int)(t * -16.0) == bin) {
-        const uint32_t at = atomicAdd(&S.n, 1u);
-        if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
-      }
-    })
-    __syncthreads();
-    const int n = (int)S.n;
-    if (S.n <= CAP) {
-      found = true;
-      const int P = pow2_at_least(n);
-      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
-      sort_list<NT>(S.list, P, true);
-      for (int base = 0; base < n; base += NT) {
-        const int i = base + tid;
-        const u64 w = i < n ? weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32))) : 0;
+  }
+  if (by_p) {
+    bool found = false;
+    u64 need = 0;
+    if (!by_k) {
+      // masses by log2 w; the bin in which the sum from above reaches what is needed is looked at closely
+      for (int b = tid; b < BINS; b += NT) S.mass[b] = 0;
+      if (tid == 0) S.key = BINS;
+      __syncthreads();
+      double sum = 0;
+      EACH_PIECE(EACH(const double t = log2_weight(sc, v[e]), w = fixed_weight(sc, t); sum += w; const int bin = (int)(t * -BINS_OCTAVE);
+                      if (bin < BINS) atomicAdd(&S.mass[bin], (u64)w);))
+      need = mass_needed(rs.p, block_total<NT>((u64)sum, S.wsum));
+      __syncthreads();
+      u64 above = 0;
+      for (int base = 0; base < BINS; base += NT) {
+        const u64 w = S.mass[base + tid];
         u64 all;
         const u64 before = above + block_scan<NT>(w, S.wsum, &all);
         if (before < need && need <= before + w) {
-          // the last one kept; how many equal it, kept and at all
-          const uint32_t key = (uint32_t)(S.list[i] >> 32);
-          int f = i, l = i;
-          while (f > 0 && (uint32_t)(S.list[f - 1] >> 32) == key) --f;
-          while (l + 1 < n && (uint32_t)(S.list[l + 1] >> 32) == key) ++l;
-          S.key = key;
-          S.n_above = l == i ? ALL : (uint32_t)(i - f + 1);
+          S.key = (uint32_t)(base + tid);
+          S.above = before;
         }
         above += all;
       }
       __syncthreads();
-      cut = S.key;
-      ties = S.n_above;
-    }
-    __syncthreads();
-  }
-  if (by_k || (by_p && !found)) {
-    // many candidates, or a bin of many: the ordered keys are searched byte by byte, the row read once for each byte;
-    // stage 0: the k-th largest key; stage 1: the key at which the mass, from above, reaches what is needed
-    for (int stage = by_k ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
-      if (stage == 1) need = mass_needed(rs.p, whole);
-      uint32_t prefix = 0, n_above = 0;
-      u64 above = 0;
-      for (int shift = 24; shift >= 0; shift -= 8) {
+      const int bin = (int)S.key;
+      above = S.above;
+      if (bin < BINS) {
+        EACH_PIECE(EACH(if ((int)(log2_weight(sc, v[e]) * -BINS_OCTAVE) == bin) {
+          const uint32_t at = atomicAdd(&S.n, 1u);
+          if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+        }))
         __syncthreads();
-        for (int b = tid; b < 256; b += NT) { S.mass[b] = 0; S.cnt[b] = 0; }
-        __syncthreads();
-        EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) {
-          const uint32_t key = key_of(v[e]);
-          if (key == 0 || key < cut || (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-          const uint32_t b = key >> shift & 255;
-          if (stage == 0) atomicAdd(&S.cnt[b], 1u);
-          else if (key > cut) atomicAdd(&S.mass[b], weight_of(sc, v[e]));
-        })
-        __syncthreads();
-        if (tid == 0) {
-          // the ties at top-k's own cut count only `ties` times
-          if (stage == 1 && ties != ALL && (shift == 24 || (cut >> (shift + 8)) == (prefix >> (shift + 8))))
-            S.mass[cut >> shift & 255] += ties * weight_of(sc, logit_of(cut));
-          u64 w = above;
-          uint32_t n = n_above;
-          int b = 255;
-          for (; b > 0; --b) {
-            if (stage == 0 ? n + S.cnt[b] >= (u64)rs.k : w + S.mass[b] >= need) break;
-            w += S.mass[b];
-            n += S.cnt[b];
+        const int n = (int)S.n;
+        if (S.n <= CAP) {
+          found = true;
+          const int P = pow2_at_least(n);
+          for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
+          sort_list<NT>(S.list, P, true);
+          for (int base = 0; base < n; base += NT) {
+            const int i = base + tid;
+            const u64 w = i < n ? (u64)weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32))) : 0;
+            u64 all;
+            const u64 before = above + block_scan<NT>(w, S.wsum, &all);
+            if (before < need && need <= before + w) {
+              // the last one kept; how many equal it, kept and at all
+              const uint32_t key = (uint32_t)(S.list[i] >> 32);
+              int f = i, l = i;
+              while (f > 0 && (uint32_t)(S.list[f - 1] >> 32) == key) --f;
+              while (l + 1 < n && (uint32_t)(S.list[l + 1] >> 32) == key) ++l;
+              S.key = key;
+              S.ties = l == i ? ALL : (uint32_t)(i - f + 1);
+            }
+            above += all;
           }
-          S.key = prefix | (uint32_t)b << shift;
-          S.above = w;
-          S.n_above = n;
-        }
-        __syncthreads();
-        prefix = S.key;
-        above = S.above;
-        n_above = S.n_above;
-      }
-      if (stage == 0) {
-        // (fewer than k logits that can be drawn: the search ends at key 0 and all of them are kept)
-        cut = prefix;
-        ties = prefix > 0 ? (uint32_t)(rs.k - n_above) : ALL;
-        if (by_p) {
-          u64 w = 0;
-          EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) if (key_of(v[e]) > cut) w += weight_of(sc, v[e]);)
-          whole = block_total<NT>(w, S.wsum);
-          if (prefix > 0) whole += ties * weight_of(sc, logit_of(cut));
-        }
-      } else {
-        const u64 w = weight_of(sc, logit_of(prefix));
-        const u64 c = w ? (need - above + w - 1) / w : 1;
-        if (prefix > cut) {
-          cut = prefix;
-          ties = c < ALL ? (uint32_t)c : ALL;
-        } else if (c < ties) {
-          ties = (uint32_t)c;
+          __syncthreads();
+          cut = logit_of(S.key);
+          ties = S.ties;
         }
       }
+      __syncthreads();
+    }
+    if (!found) {
+      // many candidates: bisection; what reaches top-k's cut has the mass of its ties there
+      const u64 tied = ties != ALL ? ties * (u64)weight_of(sc, cut) : 0;
+      const auto mass = [&](float f) { return ties == ALL || f > cut ? mass_from(f) : (cut < m ? mass_from(above_of(cut)) : 0) + tied; };
+      need = mass_needed(rs.p, mass(cut));
+      uint32_t a = key_of(cut), b = key_of(m);
+      for (int step = 0; a < b; ++step) {
+        const uint32_t k = between(a, b, step);
+        if (mass(logit_of(k)) >= need) a = k; else b = k - 1;
+      }
+      const float f = logit_of(a);
+      const u64 c = ties_needed(need - (f < m ? mass_from(above_of(f)) : 0), (u64)weight_of(sc, f));
+      if (f > cut || ties == ALL || c < ties) ties = c < ALL ? (uint32_t)c : ALL;
+      cut = f;
     }
   }
 
   // ---- by index: the waves' shares of the ties, then of the mass; the wave in whose share the sum passes walks it again
   __syncthreads();
-  uint32_t eq = 0;                         // ties before this wave's share
+  uint32_t eq = 0;                           // ties before this wave's share
   if (ties != ALL) {
     uint32_t n = 0;
-    EACH_PIECE(_Pragma("unroll") for (int e = 0; e < VEC; ++e) n += key_of(v[e]) == cut;)
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    EACH_PIECE(EACH(n += v[e] == cut;))
+    n = across<64, Add>(n);
     if (lane == 0) S.wcnt[wave] = n;
     __syncthreads();
     for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
   }
-  u64 mass = 0, target = 0, run = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    uint32_t e0 = eq;
-    for (int64_t i0 = lo; i0 < hi; i0 += 64) {
-      float v[VEC];
-      const int64_t i = i0 + lane;
-      if (i < hi) row.load(i, v);
-      else
-        for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
-      uint32_t tie = 0;                    // ties before this lane's piece
-      if (ties != ALL) {
-        uint32_t n = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n += key_of(v[e]) == cut;
-        uint32_t inc = n;
-        for (int o = 1; o < 64; o <<= 1) {
-          const uint32_t up = __shfl_up(inc, o);
-          if (lane >= o) inc += up;
-        }
-        tie = e0 + inc - n;
-        e0 += __shfl(inc, 63);
-      }
-      u64 w[VEC], sum = 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint32_t key = key_of(v[e]);
-        w[e] = 0;
-        if (key == 0 || key < cut || (key == cut && ties != ALL && tie++ >= ties)) continue;
-        const double t = log2_weight(sc, v[e]);
-        if (t >= rs.tmin) w[e] = fixed_weight(sc, t);
-        sum += w[e];
-      }
-      if (pass == 0) {
-        mass += sum;
-        continue;
-      }
-      u64 inc = sum;
-      for (int o = 1; o < 64; o <<= 1) {
-        const u64 up = __shfl_up(inc, o);
-        if (lane >= o) inc += up;
-      }
-      u64 before = run + inc - sum;
-      if (before <= target && target < before + sum) {
-        int at = 0;
-        for (; at < VEC - 1 && before + w[at] <= target; ++at) before += w[at];
-        out[r] = row.first(i) + at;
-      }
-      run += __shfl(inc, 63);
-      if (run > target) return;
+  // the kept weights of a piece
+  const auto kept = [&](const float (&v)[VEC], uint32_t& e0, double (&w)[VEC]) {
+    double sum = 0;
+    float b = -INFINITY;
+    EACH(w[e] = 0; b = fmaxf(b, v[e]);)
+    if (!__any(b >= cut)) return sum;
+    uint32_t tie = 0;                        // ties before this lane's piece
+    if (ties != ALL) {
+      uint32_t n = 0;
+      EACH(n += v[e] == cut;)
+      tie = e0 + lanes_before<64>(n, lane);
+      e0 += across<64, Add>(n);
     }
-    if (pass == 1) return;
-    for (int o = 32; o > 0; o >>= 1) mass += __shfl_xor(mass, o);
-    if (lane == 0) S.wsum[wave] = mass;
-    __syncthreads();
-    u64 all = 0;
-    for (int w = 0; w < NW; ++w) {
-      if (w < wave) run += S.wsum[w];
-      all += S.wsum[w];
+    EACH(const double t = log2_weight(sc, v[e]);
+         const bool in = (v[e] > cut || (v[e] == cut && (ties == ALL || tie++ < ties))) && t >= rs.tmin;
+         w[e] = in ? fixed_weight(sc, t) : 0.0; sum += w[e];)
+    return sum;
+  };
+  double mass = 0;
+  uint32_t e0 = eq;
+  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+    float v[VEC];
+    double w[VEC];
+    if (i0 + lane < hi) row.load(i0 + lane, v);
+    else EACH(v[e] = -INFINITY;)
+    if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
+    mass += kept(v, e0, w);
+  }
+  const u64 share = across<64, Add>((u64)mass);
+  if (lane == 0) S.wsum[wave] = share;
+  __syncthreads();
+  u64 run = 0, all = 0;
+  for (int w = 0; w < NW; ++w) {
+    if (w < wave) run += S.wsum[w];
+    all += S.wsum[w];
+  }
+  const u64 target = target_of(uu, all);
+  if (!(run <= target && target < run + share)) return;
+  e0 = eq;
+  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+    float v[VEC];
+    double w[VEC];
+    if (i0 + lane < hi) row.load(i0 + lane, v);
+    else EACH(v[e] = -INFINITY;)
+    if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
+    const u64 sum = (u64)kept(v, e0, w), pieces = across<64, Add>(sum);
+    if (run + pieces <= target) {
+      run += pieces;
+      continue;
     }
-    target = target_of(u[r], all);
-    if (!(run <= target && target < run + mass)) return;
+    u64 before = run + lanes_before<64>(sum, lane);
+    if (before <= target && target < before + sum) {
+      int at = 0;
+      EACH(before += (u64)w[e]; at += before <= target;)
+      out[r] = row.first(i0 + lane) + at;
+    }
+    return;
   }
 #undef EACH_PIECE
+#undef ONE_BY_ONE
+#undef EACH
 }
 
 template <typename T>
@@ -675,22 +707,21 @@ int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const
 #define GROUP_(G, E)                                                                                                                             \
   hipLaunchKernelGGL((sample_group_kernel<T, G, E>), dim3((unsigned)cdiv64(rows, 256 / G)), dim3(256), 0, s, rows, (int)V, (int)cdiv64(V, G), x, ld, \
                      st, F, u, out)
-  if (V <= 16) {
-    GROUP_(4, 4);
-  } else if (V <= 64) {
-    GROUP_(4, 16);
-  } else if (V <= 256) {
-    GROUP_(16, 16);
-  } else if (V <= 1024) {
-    GROUP_(64, 16);
-  } else if (V <= 2048) {
-    GROUP_(64, 32);
+  if (V <= 16) GROUP_(4, 4);
+  else if (V <= 32) GROUP_(4, 8);
+  else if (V <= 48) GROUP_(4, 12);
+  else if (V <= 64) GROUP_(4, 16);
+  else if (V <= 128) GROUP_(16, 8);
+  else if (V <= 256) GROUP_(16, 16);
+  else if (V <= 512) GROUP_(64, 8);
+  else if (V <= 1024) GROUP_(64, 16);
+  else if (V <= 1536) GROUP_(64, 24);
+  else if (V <= 2048) GROUP_(64, 32);
 #undef GROUP_
-  } else if (V <= 16384) {
+  else if (V <= 16384)
     hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, x, ld, st, F, u, out);
-  } else {
+  else
     hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, rows, V, x, ld, st, F, u, out);
-  }
   TAD_LAUNCH_CHECK();
   return TAD_OK;
 }
@@ -711,7 +742,7 @@ extern "C" int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, in
   TAD_CHECK(logits && u && out, "tad_sample_tokens: null pointer");
   int lg = 0;
   while (((int64_t)1 << lg) < V) ++lg;
-  const int F = 62 - lg < 44 ? 62 - lg : 44;
+  const int whole = V <= 2048 ? 53 : 62, F = whole - lg < 44 ? whole - lg : 44;       // bits of the largest sum
   const Settings st = {temperature, top_p, min_p, top_k, temperature_rows, top_p_rows, min_p_rows, top_k_rows};
   hipStream_t s = (hipStream_t)stream;
   return dtype == TAD_F32 ? launch_sample<float>(rows, V, logits, ld, st, F, u, out, s) : launch_sample<bf16_t>(rows, V, logits, ld, st, F, u, out, s);
