@@ -299,7 +299,8 @@ def check_sample(ops, dev, logits, u, T, k, p, m, some=0.98):
 
 
 SETTINGS = [(1.0, 0, 1.0, 0.0), (0.8, 50, 0.95, 0.02), (1.3, 0, 0.9, 0.0), (1.0, 7, 1.0, 0.0), (0.7, 0, 1.0, 0.05), (0.0, 0, 1.0, 0.0), (2.0, 300, 0.5, 0.0),
-            (1.0, 1, 0.3, 0.5), (1.0, 0, 0.0, 0.0), (1.0, 0, 0.999, 1.0)]
+            (1.0, 1, 0.3, 0.5), (1.0, 0, 0.0, 0.0), (1.0, 0, 0.999, 1.0), (1.0, 1500, 1.0, 0.0), (1.2, 1500, 0.95, 0.0), (30.0, 3000, 0.6, 0.0),
+            (50.0, 0, 0.7, 0.5), (0.05, 2000, 0.999, 0.0)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

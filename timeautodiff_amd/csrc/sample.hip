@@ -38,28 +38,28 @@ struct Scale {
 };
 // log2 of w; NaN logits, and -inf whatever T is, count as 2^-100
 __device__ __forceinline__ double log2_weight(const Scale& s, float l) { return fmax(((double)l - (double)s.m) * s.c, -100.0); }
-// 2^t in units of 2^-F, rounded to a whole number (0 from about t = -F - 1 down): 2^n times the series of 2^f = e^(f ln 2),
-// |f| <= 1/2, whose first term left out is below 2^-52
+// 2^t in units of 2^-F, rounded to a whole number (0 from about t = -F - 1 down): 2^n 2^f, n the whole number next to t, by an
+// addition that leaves n + F in the low bits, and 2^f = 1 + f g(f), |f| <= 1/2, g the polynomial that meets (2^f - 1) / f at the
+// ten Chebyshev points there: off by less than 2^-50
 __device__ __forceinline__ double fixed_weight(const Scale& s, double t) {
-  constexpr double L = 0.6931471805599453094;
-  constexpr double L2 = L * L, L3 = L2 * L, L4 = L2 * L2, L5 = L4 * L, L6 = L4 * L2, L7 = L6 * L, L8 = L4 * L4, L9 = L8 * L, L10 = L8 * L2, L11 = L10 * L,
-                   L12 = L8 * L4;
-  const double n = rint(t), f = t - n;
-  double p = L12 / 479001600;
-  p = __builtin_fma(p, f, L11 / 39916800);
-  p = __builtin_fma(p, f, L10 / 3628800);
-  p = __builtin_fma(p, f, L9 / 362880);
-  p = __builtin_fma(p, f, L8 / 40320);
-  p = __builtin_fma(p, f, L7 / 5040);
-  p = __builtin_fma(p, f, L6 / 720);
-  p = __builtin_fma(p, f, L5 / 120);
-  p = __builtin_fma(p, f, L4 / 24);
-  p = __builtin_fma(p, f, L3 / 6);
-  p = __builtin_fma(p, f, L2 / 2);
-  p = __builtin_fma(p, f, L);
+  const double magic = 6755399441055744.0 + (double)s.F, r = t + magic, f = t - (r - magic);
+  double p = 7.070977866508139e-09;
+  p = __builtin_fma(p, f, 1.0205905413765595e-07);
+  p = __builtin_fma(p, f, 1.3215451633221434e-06);
+  p = __builtin_fma(p, f, 1.5252672924850737e-05);
+  p = __builtin_fma(p, f, 0.00015403530424776529);
+  p = __builtin_fma(p, f, 0.0013333558200794592);
+  p = __builtin_fma(p, f, 0.009618129107618665);
+  p = __builtin_fma(p, f, 0.05550410866465167);
+  p = __builtin_fma(p, f, 0.24022650695910075);
+  p = __builtin_fma(p, f, 0.6931471805599462);
   p = __builtin_fma(p, f, 1.0);
-  return rint(__builtin_amdgcn_ldexp(p, (int)n + s.F));
+  const u64 b = __builtin_bit_cast(u64, p);
+  const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)__builtin_bit_cast(u64, r) << 20);
+  return rint(__builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b));
 }
+// a whole number below 2^52 as an integer
+__device__ __forceinline__ u64 whole_number(double w) { return __builtin_bit_cast(u64, w + 4503599627370496.0) & 0xfffffffffffffull; }
 __device__ __forceinline__ double weight_of(const Scale& s, float l) { return fixed_weight(s, log2_weight(s, l)); }
 // sum + w where `in`: one move and one multiply-add
 __device__ __forceinline__ double add_if(bool in, double w, double sum) { return __builtin_fma(in ? 1.0 : 0.0, w, sum); }
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
 }
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
-constexpr int BINS = 1024, BINS_OCTAVE = 64;       // of log2 w, down to 2^-16
+constexpr int BINS = 512, BINS_OCTAVE = 32;        // of log2 w, down to 2^-16
 constexpr int PAIRS = 256;                         // candidates that are compared each with each
 
 struct Candidate {
@@ -284,14 +284,15 @@ struct RowState {
   static constexpr int NW = NT / 64, CAP = 1024;
   u64 list[CAP];
   union {
-    u64 mass[BINS];
+    u64 mass[NW][BINS];
     Candidate pair[PAIRS];
   };
+  uint32_t cnt[BINS];
   u64 wsum[NW];
   uint32_t wcnt[NW];
   float wmax[NW], wmin[NW];
-  uint32_t n, key, ties;
-  u64 above;
+  uint32_t n, n_above, key, ties, at;
+  u64 above, upto;
   double total;
 };
 
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       u64 whole = 0;
       if (by_p) {
         u64 w = 0;
-        for (int i = tid; i < nk; i += NT) w += (u64)weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)));
+        for (int i = tid; i < nk; i += NT) w += whole_number(weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32))));
         whole = block_total<NT>(w, S.wsum);
       }
       const u64 need = by_p ? mass_needed(rs.p, whole) : ~0ull;
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       for (int base = 0; base < nk; base += NT) {
         const int i = base + tid;
         const double t = i < nk ? log2_weight(sc, logit_of((uint32_t)(S.list[i] >> 32))) : -100.0;
-        const u64 w = i < nk ? (u64)fixed_weight(sc, t) : 0;
+        const u64 w = i < nk ? whole_number(fixed_weight(sc, t)) : 0;
         u64 sum;
         const u64 before = above + block_scan<NT>(w, S.wsum, &sum);
         const bool keep = i < nk && before < need && t >= rs.tmin;
@@ -507,7 +508,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       u64 run = 0;
       for (int base = 0; base < (int)nkept; base += NT) {
         const int i = base + tid;
-        const u64 w = i < (int)nkept ? (u64)weight_of(sc, logit_of((uint32_t)S.list[i])) : 0;
+        const u64 w = i < (int)nkept ? whole_number(weight_of(sc, logit_of((uint32_t)S.list[i]))) : 0;
         u64 sum;
         const u64 before = run + block_scan<NT>(w, S.wsum, &sum);
         if (before <= target && target < before + w) out[r] = (int64_t)(S.list[i] >> 32);
@@ -516,185 +517,253 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       return;
     }
     __syncthreads();
-    if (tid == 0) S.n = 0;
   }
 
   // ---- the cut: every logit above `cut`, and the first `ties` (by index) that equal it (ALL: no need to count them)
   constexpr uint32_t ALL = UINT_MAX;
   float cut = -LARGEST;
   uint32_t ties = ALL;
-  // how many logits reach f, and how many of them equal it; the mass of what reaches f (with top-k's ties, if f is its cut)
-  const auto count = [&](float f) {
-    uint32_t n = 0;
-    EACH_PIECE(EACH(n += v[e] >= f;))
-    return block_total<NT>(n, S.wcnt);
-  };
-  const auto mass_from = [&](float f) {
-    double w = 0;
-    ONE_BY_ONE(float b = -INFINITY; EACH(b = fmaxf(b, v[e]);) if (__any(b >= f)) EACH(w = add_if(v[e] >= f, weight_of(sc, v[e]), w);))
-    return block_total<NT>((u64)w, S.wsum);
-  };
-  const auto above_of = [](float f) { return logit_of(key_of(f) + 1); };      // the next larger value
-  if (by_k) {
-    const uint32_t n = count(-LARGEST);
-    if (n > rs.k) {
-      const uint32_t want = (uint32_t)rs.k;
-      uint32_t a = key_of(-LARGEST), b = key_of(m), c = n;
-      for (int step = 0; a < b && c != want; ++step) {
-        const uint32_t k = between(a, b, step), got = count(logit_of(k));
-        if (got >= want) { a = k; c = got; } else b = k - 1;
-      }
-      cut = logit_of(a);
-      if (c != want) ties = want - (cut < m ? count(above_of(cut)) : 0);
-    }
-  }
-  if (by_p) {
-    bool found = false;
-    u64 need = 0;
-    if (!by_k) {
-      // masses by log2 w; the bin in which the sum from above reaches what is needed is looked at closely
-      for (int b = tid; b < BINS; b += NT) S.mass[b] = 0;
-      if (tid == 0) S.key = BINS;
-      __syncthreads();
-      double sum = 0;
-      EACH_PIECE(EACH(const double t = log2_weight(sc, v[e]), w = fixed_weight(sc, t); sum += w; const int bin = (int)(t * -BINS_OCTAVE);
-                      if (bin < BINS) atomicAdd(&S.mass[bin], (u64)w);))
-      need = mass_needed(rs.p, block_total<NT>((u64)sum, S.wsum));
-      __syncthreads();
+  bool shares = false;                       // S.wsum holds the kept mass of every wave's share
+  if (by_k || by_p) {
+    // masses, and for top-k numbers, by log2 w: the bin in which what is wanted is reached is gathered, sorted and searched
+    for (int b = tid; b < NW * BINS; b += NT) S.mass[0][b] = 0;
+    for (int b = tid; b < BINS; b += NT) S.cnt[b] = 0;
+    __syncthreads();
+    double sum = 0;
+    uint32_t number = 0;
+    ONE_BY_ONE(EACH(const double t = log2_weight(sc, v[e]), w = fixed_weight(sc, t); sum += w; number += v[e] > -INFINITY;
+                    const int bin = (int)(t * -BINS_OCTAVE);
+                    if (bin < BINS) {
+                      atomicAdd(&S.mass[wave][bin], whole_number(w));
+                      if (by_k) atomicAdd(&S.cnt[bin], 1u);
+                    }))
+    u64 whole = block_total<NT>((u64)sum, S.wsum);
+    const uint32_t drawable = block_total<NT>(number, S.wcnt);
+    // the bin where the running number (or mass) reaches what is wanted, with what lies above it; BINS: none does
+    const auto find = [&](bool by_number, u64 want) {
       u64 above = 0;
+      uint32_t n_above = 0;
+      __syncthreads();
+      if (tid == 0) S.key = BINS;
       for (int base = 0; base < BINS; base += NT) {
-        const u64 w = S.mass[base + tid];
+        const int b = base + tid;
+        u64 w = 0, all;
+        uint32_t n = 0, n_all;
+        if (b < BINS) {
+          for (int i = 0; i < NW; ++i) w += S.mass[i][b];
+          n = S.cnt[b];
+        }
+        const u64 before = above + block_scan<NT>(w, S.wsum, &all);
+        const uint32_t n_before = n_above + block_scan<NT>(n, S.wcnt, &n_all);
+        if (by_number ? n_before < want && want <= n_before + n : before < want && want <= before + w) {
+          S.key = (uint32_t)b;
+          S.above = before;
+          S.n_above = n_before;
+        }
+        above += all;
+        n_above += n_all;
+      }
+      __syncthreads();
+      return (int)S.key;
+    };
+    // the logits of a bin, falling; false if they are too many
+    const auto gather = [&](int bin) {
+      if (tid == 0) S.n = 0;
+      __syncthreads();
+      EACH_PIECE(EACH(if ((int)(log2_weight(sc, v[e]) * -BINS_OCTAVE) == bin) {
+        const uint32_t at = atomicAdd(&S.n, 1u);
+        if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+      }))
+      __syncthreads();
+      if (S.n > CAP) return false;
+      const int n = (int)S.n, P = pow2_at_least(n);
+      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
+      sort_list<NT>(S.list, P, true);
+      return true;
+    };
+    // the cut at the list's entry at which the number (or the mass, S.above of it above the list) reaches `want`
+    const auto cut_in_list = [&](bool by_number, u64 want) {
+      const int n = (int)S.n;
+      u64 above = S.above;
+      const uint32_t n_above = S.n_above;
+      for (int base = 0; base < n; base += NT) {
+        const int i = base + tid;
+        const u64 w = i < n ? whole_number(weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)))) : 0;
         u64 all;
         const u64 before = above + block_scan<NT>(w, S.wsum, &all);
-        if (before < need && need <= before + w) {
-          S.key = (uint32_t)(base + tid);
-          S.above = before;
+        if (i < n && (by_number ? n_above + i + 1 == want : before < want && want <= before + w)) {
+          const uint32_t key = (uint32_t)(S.list[i] >> 32);
+          int f = i;
+          while (f > 0 && (uint32_t)(S.list[f - 1] >> 32) == key) --f;
+          S.key = key;
+          S.ties = i + 1 < n && (uint32_t)(S.list[i + 1] >> 32) == key ? (uint32_t)(i - f + 1) : ALL;
+          S.at = (uint32_t)i;
+          S.upto = before + w;
         }
         above += all;
       }
       __syncthreads();
-      const int bin = (int)S.key;
-      above = S.above;
-      if (bin < BINS) {
-        EACH_PIECE(EACH(if ((int)(log2_weight(sc, v[e]) * -BINS_OCTAVE) == bin) {
-          const uint32_t at = atomicAdd(&S.n, 1u);
-          if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
-        }))
-        __syncthreads();
-        const int n = (int)S.n;
-        if (S.n <= CAP) {
-          found = true;
-          const int P = pow2_at_least(n);
-          for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
-          sort_list<NT>(S.list, P, true);
-          for (int base = 0; base < n; base += NT) {
-            const int i = base + tid;
-            const u64 w = i < n ? (u64)weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32))) : 0;
-            u64 all;
-            const u64 before = above + block_scan<NT>(w, S.wsum, &all);
-            if (before < need && need <= before + w) {
-              // the last one kept; how many equal it, kept and at all
-              const uint32_t key = (uint32_t)(S.list[i] >> 32);
-              int f = i, l = i;
-              while (f > 0 && (uint32_t)(S.list[f - 1] >> 32) == key) --f;
-              while (l + 1 < n && (uint32_t)(S.list[l + 1] >> 32) == key) ++l;
-              S.key = key;
-              S.ties = l == i ? ALL : (uint32_t)(i - f + 1);
-            }
-            above += all;
-          }
-          __syncthreads();
-          cut = logit_of(S.key);
-          ties = S.ties;
-        }
+      cut = logit_of(S.key);
+      ties = S.ties;
+    };
+    int bin = BINS;
+    bool found = true;
+    if (by_k && drawable > rs.k) {
+      bin = find(true, (u64)rs.k);
+      found = bin < BINS && gather(bin);
+      if (found) {
+        cut_in_list(true, (u64)rs.k);
+        whole = S.upto;
       }
+    }
+    if (by_p && found) {
+      const u64 need = mass_needed(rs.p, whole);
+      const int kbin = bin;
+      bin = find(false, need);          // (top-k's own bin again: the list is there)
+      found = bin < BINS && (bin == kbin || gather(bin));
+      if (found) cut_in_list(false, need);
+    }
+    if (found && bin < BINS && rs.tmin == -INFINITY) {
+      // the shares' kept masses: whole bins above the cut's, and the list up to it
+      shares = true;
+      u64 w = 0;
+      for (int b = lane; b < bin; b += 64) w += S.mass[wave][b];
+      w = across<64, Add>(w);
       __syncthreads();
+      if (lane == 0) S.wsum[wave] = w;
+      __syncthreads();
+      for (int i = tid; i <= (int)S.at; i += NT) {
+        const int64_t piece = ((int64_t)(uint32_t)~(uint32_t)S.list[i] + row.a) / VEC;
+        atomicAdd(&S.wsum[piece / seg], whole_number(weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)))));
+      }
     }
     if (!found) {
-      // many candidates: bisection; what reaches top-k's cut has the mass of its ties there
-      const u64 tied = ties != ALL ? ties * (u64)weight_of(sc, cut) : 0;
-      const auto mass = [&](float f) { return ties == ALL || f > cut ? mass_from(f) : (cut < m ? mass_from(above_of(cut)) : 0) + tied; };
-      need = mass_needed(rs.p, mass(cut));
-      uint32_t a = key_of(cut), b = key_of(m);
-      for (int step = 0; a < b; ++step) {
-        const uint32_t k = between(a, b, step);
-        if (mass(logit_of(k)) >= need) a = k; else b = k - 1;
+      // a bin of many, or none: bisection over the row
+      cut = -LARGEST;
+      ties = ALL;
+      const auto above_of = [](float f) { return logit_of(key_of(f) + 1); };      // the next larger value
+      const auto count = [&](float f) {
+        uint32_t n = 0;
+        EACH_PIECE(EACH(n += v[e] >= f;))
+        return block_total<NT>(n, S.wcnt);
+      };
+      const auto mass_from = [&](float f) {
+        double w = 0;
+        ONE_BY_ONE(float b = -INFINITY; EACH(b = fmaxf(b, v[e]);) if (__any(b >= f)) EACH(w = add_if(v[e] >= f, weight_of(sc, v[e]), w);))
+        return block_total<NT>((u64)w, S.wsum);
+      };
+      if (by_k && drawable > rs.k) {
+        const uint32_t want = (uint32_t)rs.k;
+        uint32_t a = key_of(-LARGEST), b = key_of(m), c = drawable;
+        for (int step = 0; a < b && c != want; ++step) {
+          const uint32_t k = between(a, b, step), got = count(logit_of(k));
+          if (got >= want) { a = k; c = got; } else b = k - 1;
+        }
+        cut = logit_of(a);
+        if (c != want) ties = want - (cut < m ? count(above_of(cut)) : 0);
       }
-      const float f = logit_of(a);
-      const u64 c = ties_needed(need - (f < m ? mass_from(above_of(f)) : 0), (u64)weight_of(sc, f));
-      if (f > cut || ties == ALL || c < ties) ties = c < ALL ? (uint32_t)c : ALL;
-      cut = f;
+      if (by_p) {
+        // what reaches top-k's cut has the mass of its ties there
+        const u64 tied = ties != ALL ? ties * whole_number(weight_of(sc, cut)) : 0;
+        const auto mass = [&](float f) { return ties == ALL || f > cut ? mass_from(f) : (cut < m ? mass_from(above_of(cut)) : 0) + tied; };
+        const u64 need = mass_needed(rs.p, mass(cut));
+        uint32_t a = key_of(cut), b = key_of(m);
+        for (int step = 0; a < b; ++step) {
+          const uint32_t k = between(a, b, step);
+          if (mass(logit_of(k)) >= need) a = k; else b = k - 1;
+        }
+        const float f = logit_of(a);
+        const u64 c = ties_needed(need - (f < m ? mass_from(above_of(f)) : 0), whole_number(weight_of(sc, f)));
+        if (f > cut || ties == ALL || c < ties) ties = c < ALL ? (uint32_t)c : ALL;
+        cut = f;
+      }
     }
   }
 
-  // ---- by index: the waves' shares of the ties, then of the mass; the wave in whose share the sum passes walks it again
-  __syncthreads();
-  uint32_t eq = 0;                           // ties before this wave's share
-  if (ties != ALL) {
-    uint32_t n = 0;
-    EACH_PIECE(EACH(n += v[e] == cut;))
-    n = across<64, Add>(n);
-    if (lane == 0) S.wcnt[wave] = n;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
-  }
-  // the kept weights of a piece
-  const auto kept = [&](const float (&v)[VEC], uint32_t& e0, double (&w)[VEC]) {
+  // ---- by index: the waves' masses, then the share in which the sum passes divided among the waves, until a wave holds it
+  const bool everything = cut == -LARGEST && rs.tmin == -INFINITY;
+  // the kept weights of a piece; tie: ties before it
+  const auto kept = [&](const float (&v)[VEC], uint32_t tie, double (&w)[VEC]) {
     double sum = 0;
-    float b = -INFINITY;
-    EACH(w[e] = 0; b = fmaxf(b, v[e]);)
-    if (!__any(b >= cut)) return sum;
-    uint32_t tie = 0;                        // ties before this lane's piece
-    if (ties != ALL) {
-      uint32_t n = 0;
-      EACH(n += v[e] == cut;)
-      tie = e0 + lanes_before<64>(n, lane);
-      e0 += across<64, Add>(n);
+    if (everything) {
+      EACH(w[e] = weight_of(sc, v[e]); sum += w[e];)
+    } else if (ties == ALL) {
+      EACH(const double t = log2_weight(sc, v[e]); w[e] = v[e] >= cut && t >= rs.tmin ? fixed_weight(sc, t) : 0.0; sum += w[e];)
+    } else {
+      EACH(const double t = log2_weight(sc, v[e]); const bool in = (v[e] > cut || (v[e] == cut && tie++ < ties)) && t >= rs.tmin;
+           w[e] = in ? fixed_weight(sc, t) : 0.0; sum += w[e];)
     }
-    EACH(const double t = log2_weight(sc, v[e]);
-         const bool in = (v[e] > cut || (v[e] == cut && (ties == ALL || tie++ < ties))) && t >= rs.tmin;
-         w[e] = in ? fixed_weight(sc, t) : 0.0; sum += w[e];)
     return sum;
   };
-  double mass = 0;
-  uint32_t e0 = eq;
-  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
-    float v[VEC];
-    double w[VEC];
-    if (i0 + lane < hi) row.load(i0 + lane, v);
-    else EACH(v[e] = -INFINITY;)
-    if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
-    mass += kept(v, e0, w);
-  }
-  const u64 share = across<64, Add>((u64)mass);
-  if (lane == 0) S.wsum[wave] = share;
-  __syncthreads();
-  u64 run = 0, all = 0;
-  for (int w = 0; w < NW; ++w) {
-    if (w < wave) run += S.wsum[w];
-    all += S.wsum[w];
-  }
-  const u64 target = target_of(uu, all);
-  if (!(run <= target && target < run + share)) return;
-  e0 = eq;
-  for (int64_t i0 = lo; i0 < hi; i0 += 64) {
-    float v[VEC];
-    double w[VEC];
-    if (i0 + lane < hi) row.load(i0 + lane, v);
-    else EACH(v[e] = -INFINITY;)
-    if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
-    const u64 sum = (u64)kept(v, e0, w), pieces = across<64, Add>(sum);
-    if (run + pieces <= target) {
-      run += pieces;
-      continue;
+  int64_t A = 0, B = row.np;
+  u64 base = 0, target = 0;
+  uint32_t tie = 0;                          // ties before piece A
+  for (bool first = true; first || B - A > 64; first = false) {
+    const int64_t share = (B - A + NW - 1) / NW, a = A + wave * share < B ? A + wave * share : B, b = a + share < B ? a + share : B;
+    uint32_t eq = 0;
+    __syncthreads();
+    if (ties != ALL) {
+      for (int64_t i = a + lane; i < b; i += 64) {
+        float v[VEC];
+        row.load(i, v);
+        EACH(eq += (infinite && v[e] == INFINITY ? LARGEST : v[e]) == cut;)
+      }
+      eq = across<64, Add>(eq);
+      if (lane == 0) S.wcnt[wave] = eq;
+      __syncthreads();
+      eq = tie;
+      for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
     }
-    u64 before = run + lanes_before<64>(sum, lane);
-    if (before <= target && target < before + sum) {
-      int at = 0;
-      EACH(before += (u64)w[e]; at += before <= target;)
-      out[r] = row.first(i0 + lane) + at;
+    if (!(first && shares)) {
+      double mass = 0;
+      for (int64_t i0 = a; i0 < b; i0 += 64) {
+        float v[VEC], most = -INFINITY;
+        double w[VEC];
+        if (i0 + lane < b) row.load(i0 + lane, v);
+        else EACH(v[e] = -INFINITY;)
+        if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
+        EACH(most = fmaxf(most, v[e]);)
+        if (!__any(most >= cut)) continue;
+        uint32_t before = 0;
+        if (ties != ALL) {
+          uint32_t n = 0;
+          EACH(n += v[e] == cut;)
+          before = eq + lanes_before<64>(n, lane);
+          eq += across<64, Add>(n);
+        }
+        mass += kept(v, before, w);
+      }
+      const u64 all = across<64, Add>((u64)mass);
+      if (lane == 0) S.wsum[wave] = all;
+      __syncthreads();
     }
-    return;
+    if (first) {
+      u64 all = 0;
+      for (int w = 0; w < NW; ++w) all += S.wsum[w];
+      target = target_of(uu, all);
+    }
+    int w = 0;
+    for (; w < NW - 1 && base + S.wsum[w] <= target; ++w) {
+      base += S.wsum[w];
+      if (ties != ALL) tie += S.wcnt[w];
+    }
+    A += w * share;
+    B = A + share < B ? A + share : B;
+  }
+  if (wave != 0) return;
+  float v[VEC];
+  double w[VEC];
+  if (A + lane < B) row.load(A + lane, v);
+  else EACH(v[e] = -INFINITY;)
+  if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
+  uint32_t n = 0;
+  EACH(n += v[e] == cut;)
+  const u64 sum = (u64)kept(v, tie + lanes_before<64>(n, lane), w);
+  u64 before = base + lanes_before<64>(sum, lane);
+  if (before <= target && target < before + sum) {
+    int at = 0;
+    EACH(before += (u64)w[e]; at += before <= target;)
+    out[r] = row.first(A + lane) + at;
   }
 #undef EACH_PIECE
 #undef ONE_BY_ONE
