@@ -375,9 +375,42 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   }
 #define EACH(...) _Pragma("unroll") for (int e = 0; e < VEC; ++e) { __VA_ARGS__ }
 
-  // the thread's largest logit, the row's, and the smallest of the threads'
+  // the thread's largest logit, the row's, and the smallest of the threads'; the thread's first H pieces stay in registers
+  // for the next look at the row
+  constexpr int H = 16;
+  typename RowPieces<T>::pack held[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    if (lo + lane + 64 * h < hi) held[h] = row.raw(lo + lane + 64 * h);
   float tm = -INFINITY;
-  EACH_PIECE(EACH(tm = fmaxf(tm, v[e]);))
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    if (lo + lane + 64 * h < hi) EACH(tm = fmaxf(tm, (float)held[h][e]);)
+  for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
+    float v[VEC];
+    row.load(i, v);
+    EACH(tm = fmaxf(tm, v[e]);)
+  }
+  // the pieces of which an element reaches f: `body` of every element (a logit, its index) of them that does
+  const auto each_from = [&](float f, const auto& body) {
+    const auto one = [&](int64_t i, const float (&v)[VEC]) {
+      float b = -INFINITY;
+      EACH(b = fmaxf(b, v[e]);)
+      if (b >= f) EACH(if (v[e] >= f) body(infinite && v[e] == INFINITY ? LARGEST : v[e], row.first(i) + e);)
+    };
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (lo + lane + 64 * h < hi) {
+        float v[VEC];
+        EACH(v[e] = (float)held[h][e];)
+        one(lo + lane + 64 * h, v);
+      }
+    for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
+      float v[VEC];
+      row.load(i, v);
+      one(i, v);
+    }
+  };
   float m = across<64, Max>(tm), least = across<64, Min>(tm > -INFINITY ? tm : INFINITY);
   if (lane == 0) {
     S.wmax[wave] = m;
@@ -396,7 +429,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   }
   if (!(rs.T > 0.0)) {
     u64 at = ~0ull;                         // the lowest index of the largest
-    EACH_PIECE(EACH(const u64 j = (u64)(row.first(i) + e); at = v[e] == m && j < at ? j : at;))
+    each_from(m, [&](float, int64_t j) { at = (u64)j < at ? (u64)j : at; });
     at = across<64, Min>(at);
     if (lane == 0) S.wsum[wave] = at;
     __syncthreads();
@@ -430,10 +463,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       }
       floor = logit_of(a);
     }
-    EACH_PIECE(EACH(if (v[e] >= floor) {
+    each_from(floor, [&](float l, int64_t j) {
       const uint32_t at = atomicAdd(&S.n, 1u);
-      if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
-    }))
+      if (at < CAP) S.list[at] = (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)j;
+    });
     __syncthreads();
     const int n = S.n < CAP + 1 ? (int)S.n : CAP + 1, nk = kk < n ? (int)kk : n;
     if (n <= PAIRS) {
