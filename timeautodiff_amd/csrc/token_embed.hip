@@ -51,34 +51,32 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
 }
 
 // ---------------------------------------------------------------- forward
-// L lanes (a power of two, at most a wave) walk the columns of one row; a wave holds 64 / L rows side by side and EF_U of
-// them one after another, whose loads are all issued before the first is used.
-constexpr int EF_U = 4;
-
-template <typename TI, typename TO, int VEC>
+// L lanes (a power of two, at most a wave) walk the columns of one row; a wave holds 64 / L rows side by side and U of them one
+// after another, whose loads are all issued before the first is used.
+template <typename TI, typename TO, int VEC, int U>
 __global__ __launch_bounds__(256) void token_embed_fwd_kernel(int64_t n, int nv, int lanes_log2, int64_t vocab, const int64_t* __restrict__ tok,
                                                               int64_t tstride, float scale, const TI* __restrict__ table, int64_t ldt,
                                                               TO* __restrict__ out, int64_t ldo) {
   const int L = 1 << lanes_log2;
-  const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;     // EF_U rows each
+  const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;     // U rows each
   const int64_t ngroups = ((int64_t)gridDim.x * 256) >> lanes_log2;
   const int lane = threadIdx.x & (L - 1);
-  int64_t row[EF_U], t[EF_U];
+  int64_t row[U], t[U];
 #pragma unroll
-  for (int u = 0; u < EF_U; ++u) {
+  for (int u = 0; u < U; ++u) {
     row[u] = group + u * ngroups;
     t[u] = row[u] < n ? tok[row[u] * tstride] : -1;
   }
   for (int c = lane; c < nv; c += L) {
-    float v[EF_U][VEC];
+    float v[U][VEC];
 #pragma unroll
-    for (int u = 0; u < EF_U; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[u][i] = 0.f;
       if ((uint64_t)t[u] < (uint64_t)vocab) load_pack<TI, VEC>(table + t[u] * ldt + (int64_t)c * VEC, v[u]);
     }
 #pragma unroll
-    for (int u = 0; u < EF_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (row[u] < n) {
         const bool live = (uint64_t)t[u] < (uint64_t)vocab;
 #pragma unroll
@@ -436,19 +434,24 @@ GradPlan grad_plan(int64_t n, int D, int dtype, bool wide) {
 template <typename TI, typename TO>
 int launch_fwd(int64_t n, int D, int64_t vocab, const int64_t* tok, int64_t tstride, float scale, const void* table, int64_t ldt, void* out,
                int64_t ldo, hipStream_t s) {
-  constexpr int V = sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4;
+  constexpr int V = sizeof(TI) + sizeof(TO) < 8 ? 8 : 4;
   const bool wide = D % V == 0 && ldt % V == 0 && ldo % V == 0 && aligned16(table) && aligned16(out);
   const int nv = wide ? D / V : D;
   int ll = 0;
   while (ll < 6 && (1 << ll) < nv) ++ll;
-  const int64_t groups = cdiv64(n, EF_U), grid = cdiv64(groups << ll, 256);
+  // four rows a lane where that still leaves every CU several waves
+  const bool many = (cdiv64(n, 4) << ll) >= 256 * 1024;
+  const int64_t grid = cdiv64(cdiv64(n, many ? 4 : 1) << ll, 256);
   TAD_CHECK(grid <= INT_MAX, "tad_token_embed_fwd: too many tokens");
-  if (wide)
-    hipLaunchKernelGGL((token_embed_fwd_kernel<TI, TO, V>), dim3((unsigned)grid), dim3(256), 0, s, n, nv, ll, vocab, tok, tstride, scale,
-                       (const TI*)table, ldt, (TO*)out, ldo);
-  else
-    hipLaunchKernelGGL((token_embed_fwd_kernel<TI, TO, 1>), dim3((unsigned)grid), dim3(256), 0, s, n, nv, ll, vocab, tok, tstride, scale,
-                       (const TI*)table, ldt, (TO*)out, ldo);
+#define FWD_(VEC, U)                                                                                                                                   \
+  hipLaunchKernelGGL((token_embed_fwd_kernel<TI, TO, VEC, U>), dim3((unsigned)grid), dim3(256), 0, s, n, nv, ll, vocab, tok, tstride, scale, (const TI*)table, \
+                     ldt, (TO*)out, ldo)
+  if (wide) {
+    if (many) FWD_(V, 4); else FWD_(V, 1);
+  } else {
+    if (many) FWD_(1, 4); else FWD_(1, 1);
+  }
+#undef FWD_
   TAD_LAUNCH_CHECK();
   return TAD_OK;
 }

@@ -941,9 +941,23 @@ def heads_to_tensor(heads, nb, nc, nn, cards, out):
 
 
 # ------------------------------------------------------------------ token family
-def _vec(t, dtype):
+# (serving calls of a few microseconds on the device: these wrappers look the current device up once and work a call's cost
+# out only for a trace)
+def _rows(t, dev):
+    """as2d for a float32, bfloat16 or int64 tensor on device ``dev`` (an index): (ptr, rows, cols, ld)."""
+    if not t.is_cuda or t.device.index != dev:
+        _chk_dev(t)
+    if t.is_contiguous() and t.dim() > 0:
+        cols = t.shape[-1]
+        return t.data_ptr(), t.numel() // cols if cols else 0, cols, cols
+    assert t.shape[-1] > 0, t.shape
+    return as2d(t, t.dtype)
+
+
+def _vec(t, dtype, dev):
     """(ptr, n, stride) of a 1-D tensor (any stride), or of a contiguous one of any shape taken as 1-D."""
-    _chk_dev(t)
+    if not t.is_cuda or t.device.index != dev:
+        _chk_dev(t)
     assert t.dtype == dtype, (t.dtype, dtype)
     if t.dim() == 1:
         return t.data_ptr(), t.shape[0], t.stride(0)
@@ -951,16 +965,25 @@ def _vec(t, dtype):
     return t.data_ptr(), t.numel(), 1
 
 
+def _per_row(t, rows, dtype, dev):
+    """Pointer to a contiguous tensor of one number per row."""
+    if not t.is_cuda or t.device.index != dev:
+        _chk_dev(t)
+    assert t.dtype == dtype and t.is_contiguous() and t.numel() == rows, (t.dtype, t.shape, t.stride(), rows)
+    return t.data_ptr()
+
+
 def token_embed_fwd(tokens, table, out, scale=1.0):
     """out[i] = scale * table[tokens[i]]: tokens int64 (1-D of any stride, or contiguous), table [V, D] and out [..., D] float32
     or bfloat16.  A token outside [0, V) is padding: a row of zeros."""
-    kp, n, ks = _vec(tokens, torch.int64)
+    dev = torch.cuda.current_device()
+    kp, n, ks = _vec(tokens, torch.int64, dev)
     assert table.dim() == 2
-    tp, V, D, ldt = as2d(table, table.dtype)
-    op, rows, Do, ldo = as2d(out, out.dtype)
+    tp, V, D, ldt = _rows(table, dev)
+    op, rows, Do, ldo = _rows(out, dev)
     assert rows == n and D == Do, (tokens.shape, table.shape, out.shape)
-    _call("tad_token_embed_fwd", n, D, V, kp, ks, float(scale), tp, _dtype(table), ldt, op, _dtype(out), ldo, _stream(),
-          cost=(float(n * D), 8.0 * n + min(n, V) * D * table.element_size() + n * D * out.element_size()))
+    cost = (0.0, 0.0) if _TRACE is None else (float(n * D), 8.0 * n + min(n, V) * D * table.element_size() + n * D * out.element_size())
+    _call("tad_token_embed_fwd", n, D, V, kp, ks, scale, tp, _dtype(table), ldt, op, _dtype(out), ldo, _stream(), cost=cost)
 
 
 def token_embed_bwd_workspace_bytes(n, D):
@@ -973,16 +996,18 @@ def token_embed_bwd(tokens, dout, dtable, scale=1.0, accumulate=True, workspace=
     fixed order; accumulate=False writes every row of dtable instead (zeros where no token names it).  dout [..., D]
     float32 or bfloat16, dtable [V, D] float32.  workspace: a uint8 tensor of token_embed_bwd_workspace_bytes(...) bytes that no
     other call in flight uses (default: allocated for the call)."""
-    kp, n, ks = _vec(tokens, torch.int64)
-    dp, rows, D, ldd = as2d(dout, dout.dtype)
-    assert dtable.dim() == 2
-    gp, V, Dg, ldg = as2d(dtable)
+    dev = torch.cuda.current_device()
+    kp, n, ks = _vec(tokens, torch.int64, dev)
+    dp, rows, D, ldd = _rows(dout, dev)
+    assert dtable.dim() == 2 and dtable.dtype == torch.float32
+    gp, V, Dg, ldg = _rows(dtable, dev)
     assert rows == n and D == Dg, (tokens.shape, dout.shape, dtable.shape)
     if workspace is None:
         workspace = torch.empty(token_embed_bwd_workspace_bytes(n, D), dtype=torch.uint8, device=dtable.device)
     assert workspace.dtype == torch.uint8 and workspace.is_contiguous()
-    _call("tad_token_embed_bwd", n, D, V, kp, ks, float(scale), dp, _dtype(dout), ldd, gp, ldg, int(bool(accumulate)), _ptr(workspace),
-          workspace.numel(), _stream(), cost=(float(n * D), 8.0 * n + n * D * dout.element_size() + 4.0 * D * (2 * min(n, V) if accumulate else V)))
+    cost = (0.0, 0.0) if _TRACE is None else (float(n * D), 8.0 * n + n * D * dout.element_size() + 4.0 * D * (2 * min(n, V) if accumulate else V))
+    _call("tad_token_embed_bwd", n, D, V, kp, ks, scale, dp, _dtype(dout), ldd, gp, ldg, 1 if accumulate else 0, _ptr(workspace), workspace.numel(),
+          _stream(), cost=cost)
 
 
 def distill_loss(logits, index, value, loss_rows, temperature=1.0, row_weight=None, grad_scale=1.0, dlogits=None):
@@ -990,26 +1015,26 @@ def distill_loss(logits, index, value, loss_rows, temperature=1.0, row_weight=No
     entries whose index lies in [0, V), p the softmax of logits[r] / tau; dlogits (optional; may be logits itself) =
     grad_scale * the gradient.  logits / dlogits [..., V] float32 or bfloat16, index int64 and value float32 [..., K],
     row_weight and loss_rows contiguous float32 of one number per row."""
-    xp, rows, V, ld = as2d(logits, logits.dtype)
-    ip, ri, K, ldi = as2d(index, torch.int64)
-    vp, rv, Kv, ldv = as2d(value)
+    dev = torch.cuda.current_device()
+    xp, rows, V, ld = _rows(logits, dev)
+    ip, ri, K, ldi = _rows(index, dev)
+    vp, rv, Kv, ldv = _rows(value, dev)
+    assert index.dtype == torch.int64 and value.dtype == torch.float32, (index.dtype, value.dtype)
     assert ri == rows and rv == rows and K == Kv and (ldi == ldv or rows == 1), (logits.shape, index.shape, index.stride(), value.shape, value.stride())
-    assert loss_rows.dtype == torch.float32 and loss_rows.is_contiguous() and loss_rows.numel() == rows
-    assert row_weight is None or (row_weight.dtype == torch.float32 and row_weight.is_contiguous() and row_weight.numel() == rows)
+    lp = _per_row(loss_rows, rows, torch.float32, dev)
+    wp = None if row_weight is None else _per_row(row_weight, rows, torch.float32, dev)
     dp, ldd = None, 0
     if dlogits is not None:
-        dp, rd, Vd, ldd = as2d(dlogits, logits.dtype)
+        assert dlogits.dtype == logits.dtype, (logits.dtype, dlogits.dtype)
+        dp, rd, Vd, ldd = _rows(dlogits, dev)
         assert rd == rows and Vd == V, (logits.shape, dlogits.shape)
-    _call("tad_distill_loss", rows, V, K, xp, _dtype(logits), ld, ip, vp, max(ldi, K), float(temperature), _ptr(row_weight), float(grad_scale),
-          _ptr(loss_rows), dp, ldd, _stream(), cost=((6.0 if dp else 3.0) * rows * V, rows * (V * logits.element_size() * (2.0 if dp else 1.0) + 12.0 * K + 8.0)))
+    cost = (0.0, 0.0) if _TRACE is None else ((6.0 if dp else 3.0) * rows * V, rows * (V * logits.element_size() * (2.0 if dp else 1.0) + 12.0 * K + 8.0))
+    _call("tad_distill_loss", rows, V, K, xp, _dtype(logits), ld, ip, vp, ldi, temperature, wp, grad_scale, lp, dp, ldd, _stream(), cost=cost)
 
 
-def _setting(v, rows, dtype):
+def _setting(v, rows, dtype, dev):
     """A setting of sample_tokens: (number, None), or (0, pointer) for a tensor of one number per row."""
-    if not isinstance(v, torch.Tensor):
-        return v, None
-    assert v.dtype == dtype and v.is_contiguous() and v.numel() == rows, (v.dtype, v.shape, rows)
-    return 0, _ptr(v)
+    return (0, _per_row(v, rows, dtype, dev)) if isinstance(v, torch.Tensor) else (v, None)
 
 
 def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -1018,11 +1043,12 @@ def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     the uniform number u[r]; see tad_sample_tokens for ties, masked rows (-1) and the order of the sum.  logits [..., V]
     float32 or bfloat16, u float32 and out int64, contiguous.  Each setting is a number or a tensor of one number per row
     (float32; top_k int32)."""
-    xp, rows, V, ld = as2d(logits, logits.dtype)
-    assert u.dtype == torch.float32 and u.is_contiguous() and u.numel() == rows and out.dtype == torch.int64 and out.is_contiguous() and out.numel() == rows
-    T, Tp = _setting(temperature, rows, torch.float32)
-    k, kp = _setting(top_k, rows, torch.int32)
-    p, pp = _setting(top_p, rows, torch.float32)
-    m, mp = _setting(min_p, rows, torch.float32)
-    _call("tad_sample_tokens", rows, V, xp, _dtype(logits), ld, float(T), Tp, int(k), kp, float(p), pp, float(m), mp, _ptr(u), _ptr(out), _stream(),
-          cost=(4.0 * rows * V, rows * (V * logits.element_size() + 12.0)))
+    dev = torch.cuda.current_device()
+    xp, rows, V, ld = _rows(logits, dev)
+    up, op = _per_row(u, rows, torch.float32, dev), _per_row(out, rows, torch.int64, dev)
+    T, Tp = _setting(temperature, rows, torch.float32, dev)
+    k, kp = _setting(top_k, rows, torch.int32, dev)
+    p, pp = _setting(top_p, rows, torch.float32, dev)
+    m, mp = _setting(min_p, rows, torch.float32, dev)
+    cost = (0.0, 0.0) if _TRACE is None else (4.0 * rows * V, rows * (V * logits.element_size() + 12.0))
+    _call("tad_sample_tokens", rows, V, xp, _dtype(logits), ld, T, Tp, k, kp, p, pp, m, mp, up, op, _stream(), cost=cost)
