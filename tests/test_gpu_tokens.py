@@ -519,3 +519,29 @@ def test_token_column_model_end_to_end(ops, dev):
         assert near < 2.0 ** -36 or int(code[r]) == want
     ops.token_embed_fwd(code, d(table), h)
     assert torch.equal(h, d(table)[code])
+
+
+def test_decoder_codes_drawn_from_its_distributions(ops, dev):
+    """DeapStack.decode_to_tensor(draw=...): the categorical columns are draws from the head outputs that ae.decoder returns,
+    the rest of the table is what it is without."""
+    from timeautodiff_amd import VAE
+    torch.manual_seed(8)
+    B, T, lat, nb, cards, nn = 9, 7, 4, 2, [3, 11, 70], 3
+    F = nb + len(cards) + nn
+    ae = VAE.DeapStack(1, nb, len(cards), nn, cards, F, 24, 2, 16, 8, lat)
+    z, mask = torch.randn(B, T, lat, device=dev) * 3, (torch.rand(B, T, F, device=dev) < 0.8).float()
+    heads = ae.decoder(z, mask)
+    plain = ae.decode_to_tensor(z, mask)
+    u = torch.rand(len(cards), B, T, device=dev)
+    got = ae.decode_to_tensor(z, mask, draw=dict(temperature=1.5, top_p=0.95, u=u))
+    keep = [c for c in range(F) if not nb <= c < nb + len(cards)]
+    assert torch.equal(got[..., keep], plain[..., keep])
+    for j, card in enumerate(cards):
+        logits = f64(heads["cats"][j]).reshape(B * T, card)
+        for r in range(B * T):
+            want, near = otok.sample(logits[r], float(u[j].reshape(-1)[r]), 1.5, 0, 0.95, 0.0)
+            assert near < 2.0 ** -36 or int(got[..., nb + j].reshape(-1)[r]) == want
+    assert bool((ae.decode_to_tensor(z, mask, draw=dict(top_k=1)) == plain).all())          # the largest alone: the argmax
+    assert not torch.equal(ae.decode_to_tensor(z, mask, draw=dict(temperature=5.0)), plain)
+    with pytest.raises(ValueError):
+        ae.decode_to_tensor(z, mask, draw=dict(u=u[:2]))

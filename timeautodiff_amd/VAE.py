@@ -100,10 +100,14 @@ class DeapStack(nn.Module):
         return eng.split_heads(heads, B, T)
 
     @ops.device_scope(lambda self, x, *a, **k: ops._first_cuda(x, self))
-    def decode_to_tensor(self, latent_feature, mask=None, cond=None):
+    def decode_to_tensor(self, latent_feature, mask=None, cond=None, *, draw=None):
         """decoder (VAE.py:193-215) followed by convert_to_tensor (process_edited.py:252-301) -- what every
         driver does with sampled latents -- without materialising the dict: [B,T,F] float32 of thresholded
-        bins, argmax codes and numericals."""
+        bins, argmax codes and numericals.
+
+        draw (no counterpart in the reference): a dict of temperature, top_k, top_p, min_p (all optional, see
+        ops.sample_tokens) and u, [n_cats, B, T] uniform numbers in [0, 1) (default: drawn on the device by torch's
+        generator): the categorical codes are drawn from the decoder's distributions instead of taken as their argmax."""
         eng = self.engine(latent_feature.device if latent_feature.is_cuda else None)
         eng.fp.version += 1
         z = self._dev_f32(latent_feature, eng)
@@ -111,6 +115,20 @@ class DeapStack(nn.Module):
         heads = eng.decoder(z, self._dev_f32(mask, eng), self._dev_f32(cond, eng) if cond is not None else None)
         out = torch.empty(B, T, eng.F, dtype=torch.float32, device=eng.device)
         ops.heads_to_tensor(heads, eng.nb, eng.nc, eng.nn, eng.cards, out.view(B * T, eng.F))
+        if draw is not None and eng.nc:
+            opt = dict(draw)
+            u = opt.pop("u", None)
+            if u is None:
+                u = torch.rand(eng.nc, B, T, device=eng.device)
+            elif tuple(u.shape) != (eng.nc, B, T):
+                raise ValueError(f"u has shape {tuple(u.shape)}, the categorical columns need {(eng.nc, B, T)}")
+            u = self._dev_f32(u, eng)
+            codes = torch.empty(B, T, dtype=torch.int64, device=eng.device)
+            col = eng.nb
+            for j, card in enumerate(eng.cards[:eng.nc]):
+                ops.sample_tokens(heads[:, col:col + card], u[j], codes, **opt)
+                out[:, :, eng.nb + j] = codes
+                col += card
         return out
 
     @ops.device_scope(lambda self, x, *a, **k: ops._first_cuda(x, self))

@@ -9,11 +9,10 @@
 #include <limits.h>
 #include <math.h>
 
+#include "lanes.h"
 #include "row_pieces.h"
 
 namespace {
-
-typedef unsigned long long u64;
 
 constexpr int MAX_K = 1024;
 constexpr float LOWEST = -3.4028234663852886e38f;
@@ -32,85 +31,98 @@ struct Args {
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---------------------------------------------------------------- short rows: G lanes of a wave per row
-// The row stays in registers (E logits a lane), statistics go across the G lanes; the teacher's q are laid into LDS by their
-// indices, as multiples of 2^-60 in 64-bit integers, so that an index that comes twice has the same sum in any order.
-template <int G>
-__device__ __forceinline__ float group_sum(float v) {
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-template <int G>
-__device__ __forceinline__ float group_max(float v) {
-  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
+// The row stays in registers (E logits a lane), statistics go across the G lanes by DPP, and the teacher's q reach their
+// columns through LDS, which only the row's own lanes touch: its order within the wave is all the synchronisation.  An index
+// that comes twice is seen by the entry whose mark at the column was overwritten; such entries add up all q of the index in
+// order and write the same sum.
+__device__ __forceinline__ void lds_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* logits, T* dlogits) {
   constexpr int R = 256 / G;                          // rows of a workgroup
-  __shared__ u64 tgt[R][G * E];
+  __shared__ uint32_t tgt[R][G * E];
   const int lane = threadIdx.x & (G - 1), slot = threadIdx.x / G;
   const int64_t r = (int64_t)blockIdx.x * R + slot;
-  const bool live = r < A.rows;
+  if (r >= A.rows) return;
   const int V = (int)A.V;
-  const T* x = logits + (live ? r : 0) * A.ld;
-  const float w = live ? (A.weight ? A.weight[r] : 1.f) : 0.f;
+  const T* x = logits + r * A.ld;
+  const int64_t* idx = A.index + r * A.ld_t;
+  const float* val = A.value + r * A.ld_t;
+  const auto entry = [&](int k) {                     // -1: none
+    const int64_t i = idx[k];
+    return (uint64_t)i < (uint64_t)V ? (int)i : -1;
+  };
+  // the lane's first entry stays in registers
+  const int i0 = lane < A.K ? entry(lane) : -1;
+  const float v0 = i0 >= 0 ? val[lane] : -INFINITY, x0 = i0 >= 0 ? (float)x[i0] : 0.f;
+  const float w = A.weight ? A.weight[r] : 1.f;
   float v[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int j = lane + e * G;
-    v[e] = j < V ? (float)x[j] : -INFINITY;
-    tgt[slot][j] = 0;
-  }
-  float m = LOWEST;
+  for (int e = 0; e < E; ++e) v[e] = lane + e * G < V ? (float)x[lane + e * G] : -INFINITY;
+  float m = LOWEST, tm = fmaxf(LOWEST, v0);
 #pragma unroll
   for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
-  m = group_max<G>(m);
-  float z = 0.f;
+  for (int k = lane + G; k < A.K; k += G)
+    if (entry(k) >= 0) tm = fmaxf(tm, val[k]);
+  m = across<G, Max>(m);
+  tm = across<G, Max>(tm);
+  const float q0 = ex2((v0 - tm) * A.c);
+  float z = 0.f, tz = q0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     v[e] = ex2((v[e] - m) * A.c);
     z += v[e];
   }
-  z = group_sum<G>(z);
-  const int64_t* idx = A.index + (live ? r : 0) * A.ld_t;
-  const float* val = A.value + (live ? r : 0) * A.ld_t;
-  float tm = LOWEST;
-  for (int k = lane; k < A.K; k += G)
-    if ((uint64_t)idx[k] < (uint64_t)V) tm = fmaxf(tm, val[k]);
-  tm = group_max<G>(tm);
-  float tz = 0.f;
-  for (int k = lane; k < A.K; k += G)
-    if ((uint64_t)idx[k] < (uint64_t)V) tz += ex2((val[k] - tm) * A.c);
-  tz = group_sum<G>(tz);
+  for (int k = lane + G; k < A.K; k += G)
+    if (entry(k) >= 0) tz += ex2((val[k] - tm) * A.c);
+  z = across<G, Add>(z);
+  tz = across<G, Add>(tz);
   const bool counts = w != 0.f && z != 0.f && tz != 0.f;
   const float itz = 1.f / tz, l2 = __log2f(tz) - __log2f(z);
-  float l = 0.f;
-  if (dlogits) __syncthreads();
-  for (int k = lane; k < A.K; k += G) {
-    const int64_t i = idx[k];
-    if ((uint64_t)i >= (uint64_t)V) continue;
-    const float a = (val[k] - tm) * A.c, q = ex2(a) * itz;
-    if (!(q > 0.f)) continue;
-    l += q * (a - ((float)x[i] - m) * A.c - l2);
-    if (dlogits) atomicAdd(&tgt[slot][i], (u64)((double)q * 1152921504606846976.0));
+  const auto term = [&](float q, float t, float s) { return q > 0.f ? q * ((t - tm) * A.c - (s - m) * A.c - l2) : 0.f; };
+  float l = i0 >= 0 ? term(q0 * itz, v0, x0) : 0.f;
+  for (int k = lane + G; k < A.K; k += G) {
+    const int i = entry(k);
+    if (i >= 0) l += term(ex2((val[k] - tm) * A.c) * itz, val[k], (float)x[i]);
   }
-  l = group_sum<G>(l);
-  if (lane == 0 && live) A.loss[r] = counts ? w * A.tau * A.tau * (l * LN2) : 0.f;
+  l = across<G, Add>(l);
+  if (lane == 0) A.loss[r] = counts ? w * A.tau * A.tau * (l * LN2) : 0.f;
   if (!dlogits) return;
-  __syncthreads();
-  if (!live) return;
+  uint32_t* mine = tgt[slot];
+  if (i0 >= 0) mine[i0] = lane;
+  for (int k = lane + G; k < A.K; k += G)
+    if (const int i = entry(k); i >= 0) mine[i] = k;
+  lds_in_order();
+  // an overwritten mark: the whole row takes the longer way
+  int twice = i0 >= 0 && mine[i0] != (uint32_t)lane;
+  for (int k = lane + G; k < A.K; k += G)
+    if (const int i = entry(k); i >= 0) twice |= mine[i] != (uint32_t)k;
+  twice = across<G, Max>(twice);
+  lds_in_order();
+#pragma unroll
+  for (int e = 0; e < E; ++e) mine[lane + e * G] = 0;
+  lds_in_order();
+  for (int k = lane; k < A.K; k += G) {
+    const int i = k == lane ? i0 : entry(k);
+    if (i < 0) continue;
+    float q = k == lane ? q0 * itz : ex2((val[k] - tm) * A.c) * itz;
+    if (twice) {
+      q = 0.f;
+      for (int o = 0; o < A.K; ++o)
+        if (entry(o) == i) q += ex2((val[o] - tm) * A.c) * itz;
+    }
+    mine[i] = __builtin_bit_cast(uint32_t, q);
+  }
+  lds_in_order();
   const float g = A.grad_scale * w * A.tau, iz = 1.f / z;
   T* d = dlogits + r * A.ldd;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = lane + e * G;
-    if (j < V) {
-      const u64 q = tgt[slot][j];
-      float t = 0.f;
-      if (q) t = (float)((double)q * (1.0 / 1152921504606846976.0));
-      d[j] = (T)(counts ? g * (v[e] * iz - t) : 0.f);
-    }
+    if (j < V) d[j] = (T)(counts ? g * (v[e] * iz - __builtin_bit_cast(float, mine[j])) : 0.f);
   }
 }
 
@@ -119,8 +131,8 @@ __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* log
 // from the row's end backwards, where the caches still hold it.
 template <int NW, bool MAX>
 __device__ __forceinline__ void block_two(float& a, float& b, float (*s)[NW]) {      // largest, or sum, of two values at once
-  a = MAX ? group_max<64>(a) : wave_sum(a);
-  b = MAX ? group_max<64>(b) : wave_sum(b);
+  a = MAX ? across<64, Max>(a) : wave_sum(a);
+  b = MAX ? across<64, Max>(b) : wave_sum(b);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     s[0][threadIdx.x >> 6] = a;
@@ -261,9 +273,13 @@ template <typename T>
 int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
 #define SHORT_(G, E) hipLaunchKernelGGL((distill_short_kernel<T, G, E>), dim3((unsigned)cdiv64(A.rows, 256 / G)), dim3(256), 0, s, A, x, d)
 #define ROW_(NT, H) hipLaunchKernelGGL((distill_row_kernel<T, NT, H>), dim3((unsigned)A.rows), dim3(NT), 0, s, A, x, d)
-  if (A.V <= 32) SHORT_(8, 4);
+  if (A.V <= 16) SHORT_(4, 4);
+  else if (A.V <= 32) SHORT_(16, 2);
+  else if (A.V <= 48) SHORT_(16, 3);
   else if (A.V <= 64) SHORT_(16, 4);
   else if (A.V <= 128) SHORT_(16, 8);
+  else if (A.V <= 256) SHORT_(64, 4);
+  else if (A.V <= 512) SHORT_(64, 8);
   else if (A.V <= 1024) SHORT_(64, 16);
   else if (A.V <= 16384) ROW_(256, 4);
   else if (A.V <= (sizeof(T) == 2 ? 65536 : 16384)) ROW_(512, 8);
