@@ -50,6 +50,17 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[VEC]) {
   *reinterpret_cast<P*>(p) = x;
 }
 
+// 16 bytes a lane, side by side, past the caches: rows of the table's gradient are not read again
+template <int VEC>
+__device__ __forceinline__ void stream_pack(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 4) {
+    const f32x4 x = {v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(p));
+  } else {
+    store_pack<float, VEC>(p, v);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 // L lanes (a power of two, at most a wave) walk the columns of one row; a wave holds 64 / L rows side by side and U of them one
 // after another, whose loads are all issued before the first is used.
@@ -229,12 +240,12 @@ __global__ __launch_bounds__(512) void sort_move_kernel(Digit d, int tiles, cons
 }
 
 // ---------------------------------------------------------------- sums over the sorted tokens
-// A wave adds the rows of S <= 64 neighbouring sorted positions, 64 * VEC columns of them, GW waves (a chunk) side by side.
+// A wave adds the rows of S <= 64 neighbouring sorted positions, 64 * VEC * M columns of them, GW waves (a chunk) side by side.
 // A run of equal tokens inside a wave's share is a finished row of dtable.  What reaches over an edge between waves of the
 // workgroup is added up in LDS, what reaches over its edges goes to the workspace (slot 0: the run that came in from the
 // left; slot 1: one that begins here and goes on) and is added up by the launch behind, always in the order of positions.
 constexpr int GW = 8;
-constexpr int ZROWS = 16;     // rows of the table a wave of the zero part looks after
+constexpr int ZROWS = 8;      // rows of the table a wave of the zero part looks after
 
 template <int VEC>
 __device__ __forceinline__ void put_row(float* dt, const float (&acc)[VEC], float scale, int accumulate) {
@@ -247,14 +258,15 @@ __device__ __forceinline__ void put_row(float* dt, const float (&acc)[VEC], floa
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] += o[i];
   }
-  store_pack<float, VEC>(dt, v);
+  if (accumulate) store_pack<float, VEC>(dt, v);
+  else stream_pack<VEC>(dt, v);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int M>
 __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int D, int64_t vocab, int S, int64_t nchunks, int ctiles, float scale,
                                                                  int accumulate, const u64* __restrict__ keys, const T* __restrict__ dout, int64_t ldd,
                                                                  float* __restrict__ dtable, int64_t ldg, float* __restrict__ part) {
-  constexpr int CT = 64 * VEC, U = 8;
+  constexpr int CT = 64 * VEC * M, U = 8;
   __shared__ __attribute__((aligned(16))) float edge[GW][2][CT];
   __shared__ uint32_t head_tok[GW], tail_tok[GW], state[GW];       // state: 1 a run came in, 2 and ends here, 4 one goes on
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -274,9 +286,9 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
     for (int r = 0; r < ZROWS; ++r) {
       if (!(todo >> r & 1)) continue;
       float* row = dtable + (v0 + r) * ldg;
-      for (int c = lane * VEC; c < D; c += CT) {
+      for (int c = lane * VEC; c < D; c += 64 * VEC) {
         float z[VEC] = {};
-        store_pack<float, VEC>(row + c, z);
+        stream_pack<VEC>(row + c, z);
       }
     }
     return;
@@ -285,7 +297,9 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
   const int c0 = (int)(blockIdx.x - chunk * ctiles) * CT, c = c0 + lane * VEC;
   const int64_t a = (chunk * GW + wave) * S;
   const int m = a < n ? (int)(n - a < S ? n - a : S) : 0;
-  const bool on = c < D;
+  bool on[M];
+#pragma unroll
+  for (int p = 0; p < M; ++p) on[p] = c + p * 64 * VEC < D;
   uint32_t st = 0;
   if (m > 0) {
     const u64 key = keys[a + (lane < m ? lane : m - 1)];
@@ -298,36 +312,42 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
     const u64 ends = __ballot(lane < live && tok != next);
     const uint32_t tok0 = __builtin_amdgcn_readfirstlane(tok);
     bool came = live > 0 && tok0 == left;
-    float acc[VEC] = {};
+    float acc[M][VEC] = {};
     for (int j0 = 0; j0 < live; j0 += U) {
-      float v[U][VEC];
+      float v[U][M][VEC];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int j = j0 + k < live ? j0 + k : live - 1;             // (the last row again, not added: the loads need no branch)
         const uint32_t pos = __builtin_amdgcn_readlane((uint32_t)key, j);
-        if (on) load_pack<T, VEC>(dout + (int64_t)pos * ldd + c, v[k]);
+#pragma unroll
+        for (int p = 0; p < M; ++p)
+          if (on[p]) load_pack<T, VEC>(dout + (int64_t)pos * ldd + c + p * 64 * VEC, v[k][p]);
       }
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int j = j0 + k;
         if (j >= live) break;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] += v[k][i];
-        if (ends >> j & 1) {
-          if (came) {
-            store_pack<float, VEC>(&edge[wave][0][lane * VEC], acc);
-            st |= 3;
-            came = false;
-          } else if (on) {
-            put_row<VEC>(dtable + (int64_t)__builtin_amdgcn_readlane(tok, j) * ldg + c, acc, scale, accumulate);
-          }
+        for (int p = 0; p < M; ++p)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+          for (int i = 0; i < VEC; ++i) acc[p][i] += v[k][p][i];
+        if (ends >> j & 1) {
+          const int64_t row = (int64_t)__builtin_amdgcn_readlane(tok, j) * ldg + c;
+#pragma unroll
+          for (int p = 0; p < M; ++p) {
+            if (came) store_pack<float, VEC>(&edge[wave][0][(p * 64 + lane) * VEC], acc[p]);
+            else if (on[p]) put_row<VEC>(dtable + row + p * 64 * VEC, acc[p], scale, accumulate);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[p][i] = 0.f;
+          }
+          if (came) st |= 3;
+          came = false;
         }
       }
     }
     if (live > 0 && !(ends >> (live - 1) & 1)) {                     // goes on to the right
-      store_pack<float, VEC>(&edge[wave][came ? 0 : 1][lane * VEC], acc);
+#pragma unroll
+      for (int p = 0; p < M; ++p) store_pack<float, VEC>(&edge[wave][came ? 0 : 1][(p * 64 + lane) * VEC], acc[p]);
       st |= came ? 1 : 4;
     }
     if (lane == 0) {
@@ -413,18 +433,18 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t COUNT_BYTES = MAX_TILES * MAX_BINS * 4;
 inline int64_t key_bytes(int64_t n) { return (n * 8 + 15) / 16 * 16; }
 
-// How the gradient is cut: S positions a wave, VEC columns a lane.
+// How the gradient is cut: S positions a wave, `packs` packs of VEC columns a lane.
 struct GradPlan {
-  int vec, S, ctiles;
+  int vec, packs, S, ctiles;
   int64_t nchunks;
 };
 GradPlan grad_plan(int64_t n, int D, int dtype, bool wide) {
   GradPlan g;
-  const int most = dtype == TAD_BF16 ? 8 : 4;
   g.vec = 1;
   if (wide)
-    while (g.vec < most && D >= 128 * g.vec) g.vec *= 2;
-  g.ctiles = (int)cdiv64(D, 64 * g.vec);
+    while (g.vec < 4 && D >= 128 * g.vec) g.vec *= 2;
+  g.packs = dtype == TAD_BF16 && g.vec == 4 && D >= 512 ? 2 : 1;
+  g.ctiles = (int)cdiv64(D, 64 * g.vec * g.packs);
   g.S = 64;
   while (g.S > 8 && cdiv64(n, g.S) * g.ctiles < 4096) g.S /= 2;
   g.nchunks = cdiv64(n, g.S * GW);
@@ -456,11 +476,11 @@ int launch_fwd(int64_t n, int D, int64_t vocab, const int64_t* tok, int64_t tstr
   return TAD_OK;
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int M>
 void launch_sum(const GradPlan& g, int64_t n, int D, int64_t vocab, float scale, int accumulate, const u64* keys, const void* dout, int64_t ldd,
                 float* dtable, int64_t ldg, float* part, hipStream_t s) {
   const int64_t grid = g.nchunks * g.ctiles + (accumulate ? 0 : cdiv64(vocab, ZROWS * GW));
-  hipLaunchKernelGGL((embed_grad_sum_kernel<T, VEC>), dim3((unsigned)grid), dim3(GW * 64), 0, s, n, D, vocab, g.S, g.nchunks, g.ctiles, scale,
+  hipLaunchKernelGGL((embed_grad_sum_kernel<T, VEC, M>), dim3((unsigned)grid), dim3(GW * 64), 0, s, n, D, vocab, g.S, g.nchunks, g.ctiles, scale,
                      accumulate, keys, (const T*)dout, ldd, dtable, ldg, part);
 }
 
@@ -505,8 +525,7 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
   TAD_CHECK(dtable && (n == 0 || (tokens && dout)), "tad_token_embed_bwd: null pointer");
   hipStream_t s = (hipStream_t)stream;
   if (n == 0) return tad_zero_2d(vocab, (int64_t)D * 4, dtable, ld_dtable * 4, stream);
-  const bool wide = ld_dtable % 4 == 0 && D % (dout_dtype == TAD_BF16 ? 8 : 4) == 0 && ld_dout % (dout_dtype == TAD_BF16 ? 8 : 4) == 0 &&
-                    aligned16(dout) && aligned16(dtable);
+  const bool wide = D % 4 == 0 && ld_dtable % 4 == 0 && ld_dout % 4 == 0 && aligned16(dout) && aligned16(dtable);
   const GradPlan g = grad_plan(n, D, dout_dtype, wide);
   const int64_t kb = key_bytes(n);
   TAD_CHECK(workspace && aligned16(workspace) && workspace_bytes >= 2 * kb + COUNT_BYTES + 2 * g.nchunks * D * 4,
@@ -535,11 +554,11 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
     }
     a = b;
   }
-#define SUM_(T, V) launch_sum<T, V>(g, n, D, vocab, scale, accumulate, a, dout, ld_dout, dtable, ld_dtable, part, s)
+#define SUM_(T, V, M) launch_sum<T, V, M>(g, n, D, vocab, scale, accumulate, a, dout, ld_dout, dtable, ld_dtable, part, s)
   if (dout_dtype == TAD_BF16) {
-    if (g.vec == 8) SUM_(bf16_t, 8); else if (g.vec == 4) SUM_(bf16_t, 4); else if (g.vec == 2) SUM_(bf16_t, 2); else SUM_(bf16_t, 1);
+    if (g.packs == 2) SUM_(bf16_t, 4, 2); else if (g.vec == 4) SUM_(bf16_t, 4, 1); else if (g.vec == 2) SUM_(bf16_t, 2, 1); else SUM_(bf16_t, 1, 1);
   } else {
-    if (g.vec == 4) SUM_(float, 4); else if (g.vec == 2) SUM_(float, 2); else SUM_(float, 1);
+    if (g.vec == 4) SUM_(float, 4, 1); else if (g.vec == 2) SUM_(float, 2, 1); else SUM_(float, 1, 1);
   }
 #undef SUM_
   TAD_LAUNCH_CHECK();
