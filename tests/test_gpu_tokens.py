@@ -116,7 +116,8 @@ def check_bwd(ops, dev, tok, dout, V, scale, accumulate, extra=0):
 @pytest.mark.parametrize("kind", ["zipf", "ragged", "same", "padding", "once"])
 @pytest.mark.parametrize("n,V,D,dtype", [(1, 1, 1, torch.float32), (63, 5, 3, torch.bfloat16), (64, 200, 64, torch.float32),
                                          (129, 17, 100, torch.bfloat16), (1000, 33, 128, torch.float32), (2400, 50, 520, torch.bfloat16),
-                                         (300, 5000, 260, torch.float32)])
+                                         (300, 5000, 260, torch.float32), (1, 2500, 5, torch.float32), (63, 2100, 3, torch.bfloat16),
+                                         (1000, 3000, 128, torch.float32), (2400, 4000, 520, torch.bfloat16)])
 def test_token_embed_bwd(ops, dev, kind, n, V, D, dtype):
     rng = np.random.default_rng(n + V + D)
     tok = bwd_tokens(kind, n, V, rng)

@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
 }
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
-constexpr int BINS = 512, BINS_OCTAVE = 32;        // of log2 w, down to 2^-16
+constexpr int BINS = 512;                          // of log2 w, down to 2^-16
 constexpr int PAIRS = 256;                         // candidates that are compared each with each
 
 struct Candidate {
@@ -327,14 +327,31 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
 #pragma unroll
   for (int h = 0; h < H; ++h)
     if (lo + lane + 64 * h < hi) held[h] = row.raw(lo + lane + 64 * h);
-  float tm = -INFINITY;
+  // top-p alone: the sum of the weights too, roughly (each thread relative to its own largest)
+  const bool guess = rs.T > 0.0 && !(rs.k > 0 && rs.k < V) && rs.p < 1.0 && V > CAP;
+  const float rough = (float)(1.4426950408889634074 / rs.T);
+  float tm = -INFINITY, tz = 0.f;
+  const auto look = [&](const float (&v)[VEC]) {
+    float b = tm;
+    EACH(b = fmaxf(b, v[e]);)
+    if (guess) {
+      const float from = fmaxf(b, -LARGEST);
+      tz *= __builtin_amdgcn_exp2f((tm - from) * rough);
+      EACH(tz += __builtin_amdgcn_exp2f((v[e] - from) * rough);)
+    }
+    tm = b;
+  };
 #pragma unroll
   for (int h = 0; h < H; ++h)
-    if (lo + lane + 64 * h < hi) EACH(tm = fmaxf(tm, (float)held[h][e]);)
+    if (lo + lane + 64 * h < hi) {
+      float v[VEC];
+      EACH(v[e] = (float)held[h][e];)
+      look(v);
+    }
   for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
     float v[VEC];
     row.load(i, v);
-    EACH(tm = fmaxf(tm, v[e]);)
+    look(v);
   }
   // the pieces of which an element reaches f: `body` of every element (a logit, its index) of them that does
   const auto each_from = [&](float f, const auto& body) {
@@ -393,9 +410,11 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     return step < 16 && k > a && k <= b ? k : a + (b - a + 1) / 2;
   };
 
-  // ---- few candidates: all that top-k can keep fits the list
-  if ((by_k && rs.k <= CAP / 2 && rs.k <= NT) || ((by_k || by_p) && V <= CAP)) {
-    const int64_t kk = by_k ? rs.k : V;
+  // ---- few candidates: all that top-k can keep fits the list; or, with top-p alone, a guess: that the largest GUESS logits
+  // hold top_p of the mass, as they do where a model is sure of its answers
+  constexpr int GUESS = 160;
+  if ((by_k && rs.k <= CAP / 2 && rs.k <= NT) || ((by_k || by_p) && V <= CAP) || guess) {
+    const int64_t kk = by_k ? rs.k : guess ? GUESS : V;
     // where kk threads' largest reach `floor`, at least kk logits do; not many more than kk are wanted
     float floor = -LARGEST;
     if (V > CAP && __syncthreads_count(tm >= least) >= kk) {
@@ -413,7 +432,25 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       if (at < CAP) S.list[at] = (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)j;
     });
     __syncthreads();
-    const int n = S.n < CAP + 1 ? (int)S.n : CAP + 1, nk = kk < n ? (int)kk : n;
+    int n = S.n < CAP + 1 ? (int)S.n : CAP + 1;
+    const int nk = kk < n && !guess ? (int)kk : n;
+    u64 whole_row = 0;
+    if (guess) {
+      // (weighed roughly first: only a guess that holds is worth the exact sum of the row; a NaN or an infinity: it does not)
+      bool good = n <= PAIRS;
+      if (good) {
+        const float some = tid < n ? __builtin_amdgcn_exp2f((logit_of((uint32_t)(S.list[tid] >> 32)) - m) * rough) : 0.f;
+        const float all = block_total<NT>(tz * __builtin_amdgcn_exp2f((tm - m) * rough), S.wmax);
+        good = block_total<NT>(some, S.wmin) > 1.001f * (float)rs.p * all;
+      }
+      if (good) {
+        double w = 0;
+        ONE_BY_ONE(EACH(w += weight_of(sc, v[e]);))
+        whole_row = block_total<NT>((u64)w, S.wsum);
+      } else {
+        n = CAP + 1;
+      }
+    }
     if (n <= PAIRS) {
       // each with each: its place and the mass above it in falling order, then the kept mass below it by index
       const bool on = tid < n;
@@ -434,20 +471,24 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
         if (rank == nk - 1) S.total = above + w;
       }
       __syncthreads();
-      const bool keep = on && rank < nk && (!by_p || above < mass_needed(rs.p, S.total)) && t >= rs.tmin;
-      if (on) S.pair[tid].w = keep ? w : 0.0;
-      __syncthreads();
-      if (!keep) return;
-      double before = 0, all = 0;
+      const double need = guess ? (double)mass_needed(rs.p, whole_row) : mass_needed(rs.p, S.total);
+      if (need <= S.total) {                   // (always, but for a guess)
+        const bool keep = on && rank < nk && (!by_p || above < need) && t >= rs.tmin;
+        if (on) S.pair[tid].w = keep ? w : 0.0;
+        __syncthreads();
+        if (!keep) return;
+        double before = 0, all = 0;
 #pragma unroll 8
-      for (int j = 0; j < n; ++j) {
-        const Candidate c = S.pair[j];
-        before = add_if((uint32_t)c.k > (uint32_t)mine, c.w, before);
-        all += c.w;
+        for (int j = 0; j < n; ++j) {
+          const Candidate c = S.pair[j];
+          before = add_if((uint32_t)c.k > (uint32_t)mine, c.w, before);
+          all += c.w;
+        }
+        const double target = target_of(uu, all);
+        if (before <= target && target < before + w) out[r] = (int64_t)(uint32_t)~(uint32_t)mine;
+        return;
       }
-      const double target = target_of(uu, all);
-      if (before <= target && target < before + w) out[r] = (int64_t)(uint32_t)~(uint32_t)mine;
-      return;
+      n = CAP + 1;
     }
     if (n <= CAP) {
       // sorted: by logit for the cut, the kept ones by index for the answer
@@ -503,14 +544,17 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   uint32_t ties = ALL;
   bool shares = false;                       // S.wsum holds the kept mass of every wave's share
   if (by_k || by_p) {
-    // masses, and for top-k numbers, by log2 w: the bin in which what is wanted is reached is gathered, sorted and searched
+    // masses, and for top-k numbers, by log2 w: the bin in which what is wanted is reached is gathered, sorted and searched.
+    // (Top-k may reach further down: to the smallest of the threads' largest; never to 2^-100, where what is not drawn stands)
+    const double depth = by_k ? fmin(fmax(-log2_weight(sc, least), 16.0), 90.0) : 16.0, per_octave = BINS / depth;
+    const auto bin_of = [&](double t) { return (int)(t * -per_octave); };
     for (int b = tid; b < NW * BINS; b += NT) S.mass[0][b] = 0;
     for (int b = tid; b < BINS; b += NT) S.cnt[b] = 0;
     __syncthreads();
     double sum = 0;
     uint32_t number = 0;
     ONE_BY_ONE(EACH(const double t = log2_weight(sc, v[e]), w = fixed_weight(sc, t); sum += w; number += v[e] > -INFINITY;
-                    const int bin = (int)(t * -BINS_OCTAVE);
+                    const int bin = bin_of(t);
                     if (bin < BINS) {
                       atomicAdd(&S.mass[wave][bin], whole_number(w));
                       if (by_k) atomicAdd(&S.cnt[bin], 1u);
@@ -548,7 +592,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     const auto gather = [&](int bin) {
       if (tid == 0) S.n = 0;
       __syncthreads();
-      EACH_PIECE(EACH(if ((int)(log2_weight(sc, v[e]) * -BINS_OCTAVE) == bin) {
+      EACH_PIECE(EACH(if (bin_of(log2_weight(sc, v[e])) == bin) {
         const uint32_t at = atomicAdd(&S.n, 1u);
         if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
       }))
