@@ -604,7 +604,7 @@ int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dty
  * gives -1; +inf counts as the largest float32 number.  Each setting is one number, or, where its _rows pointer is given, a number
  * per row (T, top_p, min_p float32, top_k int32; there T not above 0 means 0, top_k below 1 means all, min_p above 1 means 1;
  * NaN: T 0, the others off).  u below 0 or NaN counts as 0, u of 1 or more gives the last kept token.  The masses are
- * whole multiples of 2^-F of the largest weight (F = 44; 62 - log2 V from 2^18 logits on, 53 - log2 V from 512 to 2048): every
+ * whole multiples of 2^-F of the largest weight (F = 44; 61 - log2 V above 2^17 logits, 53 - log2 V from 512 to 2048): every
  * sum is exact. */
 int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, int dtype, int64_t ld, double temperature, const float* temperature_rows,
                       int64_t top_k, const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,

@@ -546,3 +546,46 @@ def test_decoder_codes_drawn_from_its_distributions(ops, dev):
     assert not torch.equal(ae.decode_to_tensor(z, mask, draw=dict(temperature=5.0)), plain)
     with pytest.raises(ValueError):
         ae.decode_to_tensor(z, mask, draw=dict(u=u[:2]))
+
+
+@pytest.mark.parametrize("dtype,V,rows", [(torch.float32, 2500, 300), (torch.bfloat16, 9000, 257), (torch.bfloat16, 60000, 260), (torch.float32, 40000, 258),
+                                          (torch.bfloat16, 70001, 5)])
+def test_sample_tokens_many_rows_and_long_ones(ops, dev, dtype, V, rows):
+    """Every size of workgroup that a row gets, for few rows and for many (a share of the rows is checked)."""
+    rng = np.random.default_rng(V)
+    logits = (torch.randn(rows, V, device=dev, generator=torch.Generator(device=dev).manual_seed(V)) * 2.5).to(dtype)
+    u = rng.random(rows) * 0.999
+    ask = np.arange(0, rows, max(1, rows // 12))
+    for T, k, p, m in [(1.0, 0, 0.9, 0.0), (0.5, 0, 0.9, 0.0), (0.9, 60, 0.95, 0.02), (1.0, 0, 1.0, 0.0), (1.0, 700, 0.99, 0.0), (0.0, 0, 1.0, 0.0)]:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+        ops.sample_tokens(logits, torch.from_numpy(u.astype(np.float32)).to(dev), out, temperature=T, top_k=k, top_p=p, min_p=m)
+        for r in ask:
+            want, near = otok.sample(f64(logits[r]), np.float32(u[r]), T, k, p, m)
+            assert near < 2.0 ** -36 or int(out[r]) == want, (T, k, p, m, r)
+
+
+@pytest.mark.parametrize("V", [150001, 300000])
+def test_sample_tokens_very_long_rows(ops, dev, V):
+    """Rows whose sums leave fewer bits to a weight (off by 2^-43 of the largest at 300000 logits, 3e5 of them: 2^-33 of the
+    sum at the very most where it is the largest alone, 2^-42 where they are alike)."""
+    rng = np.random.default_rng(V)
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.from_numpy(rng.standard_normal((3, V)) * 2.5).to(dev, dtype)
+        u = rng.random(3)
+        for T, k, p, m in SETTINGS:
+            check_sample(ops, dev, logits, u, T, k, p, m, some=0.6)
+
+
+@pytest.mark.parametrize("V", [3000, 20000])
+def test_sample_tokens_of_peaked_rows(ops, dev, V):
+    """Rows where a few logits hold the mass, also at one end of the row, with top-p alone and with everything."""
+    rng = np.random.default_rng(V)
+    rows = 12
+    x = rng.standard_normal((rows, V))
+    x[:, :5] += 9.0
+    x[3:6, V - 3:] += 12.0
+    x[6, 77] = 60.0
+    x[7] = np.floor(x[7])                       # few values, many ties
+    for dtype in (torch.float32, torch.bfloat16):
+        for s in SETTINGS:
+            check_sample(ops, dev, torch.from_numpy(x).to(dev, dtype), rng.random(rows) * 0.999, *s, some=0.8)

@@ -5,7 +5,7 @@
 //   w, by index, exceeds u times their sum.  Ties go to the lowest index.
 //
 // The answer is an index that a sum decides, so the sums are exact: every w is rounded once to a whole multiple of 2^-F (F =
-// 44 for rows of up to 512 logits and of 2049 to 2^18, else a few less) and added as a whole number, in float64 where all
+// 44 for rows of up to 512 logits and of 2049 to 2^17, else a few less) and added as a whole number, in float64 where all
 // of a sum fits its 53 bits and in 64-bit integers beyond.  The order of additions then changes nothing, and the answer is the
 // real numbers' unless u lies within about 2^-40 of a border.  Float64 fused multiply-adds issue at the rate of float32 ones
 // here, so such a weight costs about 20 instructions.
@@ -809,10 +809,18 @@ int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const
   else if (V <= 1536) GROUP_(64, 24);
   else if (V <= 2048) GROUP_(64, 32);
 #undef GROUP_
-  else if (V <= 16384)
-    hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, s, rows, V, x, ld, st, F, u, out);
-  else
-    hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, rows, V, x, ld, st, F, u, out);
+  else {
+    // One workgroup per row.  Up to a row for every CU the largest that the row feeds is the fastest (64 x 131072 bf16: 45 / 26 / 21
+    // us with 256 / 512 / 1024 threads; 1 x 32000: 16 / 14 / 15); with more rows small workgroups wait for each other's
+    // barriers less (4096 x 8000 bf16: 70 / 146 / 209 us; 1024 x 32000: 37 / 50 / 66; 512 x 65536: 35 / 33 / 43).
+    const int64_t bytes = V * (int64_t)sizeof(T);
+    const bool many = rows > 256;
+#define ROW_(NT) hipLaunchKernelGGL((sample_row_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, s, rows, V, x, ld, st, F, u, out)
+    if (many && bytes <= 98304) ROW_(256);
+    else if (bytes <= (many ? 1 << 20 : 131072)) ROW_(512);
+    else ROW_(1024);
+#undef ROW_
+  }
   TAD_LAUNCH_CHECK();
   return TAD_OK;
 }
@@ -833,7 +841,7 @@ extern "C" int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, in
   TAD_CHECK(logits && u && out, "tad_sample_tokens: null pointer");
   int lg = 0;
   while (((int64_t)1 << lg) < V) ++lg;
-  const int whole = V <= 2048 ? 53 : 62, F = whole - lg < 44 ? whole - lg : 44;       // bits of the largest sum
+  const int whole = V <= 2048 ? 53 : 61, F = whole - lg < 44 ? whole - lg : 44;       // bits of the row's largest sum (a thread's: 53)
   const Settings st = {temperature, top_p, min_p, top_k, temperature_rows, top_p_rows, min_p_rows, top_k_rows};
   hipStream_t s = (hipStream_t)stream;
   return dtype == TAD_F32 ? launch_sample<float>(rows, V, logits, ld, st, F, u, out, s) : launch_sample<bf16_t>(rows, V, logits, ld, st, F, u, out, s);
