@@ -575,7 +575,8 @@ int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, 
 /* Its gradient: dtable[v, :] = (accumulate: +=) scale * sum over the i with tokens[i * tok_stride] = v of dout[i, :]; dout
  * [n, D] float32 or bf16, dtable [vocab, D] float32.  Without accumulate every row of dtable is written (zeros where no token
  * names it); with it the rows that no token names are not touched.  Padding tokens have no share.  The sums are float32 in a
- * fixed order (tokens sorted, equal ones by position): the same bits from every call.  n < 2^31, vocab < 2^31 - 1.
+ * fixed order that the tokens alone decide: the same bits from every call.  n < 2^31, vocab < 2^31 - 1, and so
+ * many that no launch has 2^32 threads (a fault of size is an error).
  * workspace: tad_token_embed_bwd_workspace_bytes(n, D) bytes, 16-byte aligned, not read before it is written; calls that
  * overlap on the device (and graphs that may) need workspaces of their own. */
 int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D);
@@ -588,7 +589,8 @@ int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, 
  *   twice has the sum of its q;  p_j = softmax of logits[r, j] / tau;  w_r = row_weight[r] (NULL: 1)
  *   loss_rows[r]  = w_r tau^2 sum_k q_k (ln q_k - ln p[index_k])
  *   dlogits[r, j] = grad_scale * d loss_rows[r] / d logits[r, j] = grad_scale w_r tau (p_j - q of j)
- * logits and dlogits [rows, V] of `dtype`, index int64 and value float32 [rows, K] (row stride ld_t).  dlogits may be NULL
+ * 1e-18 <= tau <= 1e18.  logits and dlogits [rows, V] of `dtype`, index int64 and value float32 [rows, K] (row stride ld_t
+ * both).  dlogits may be NULL
  * (the loss alone) or the logits' own storage (same row stride).  Statistics and sums are float32.  The loss and the gradient
  * of a row are 0 where its weight is 0 (whatever else it holds), where it has no entry with a value above -inf, and where no
  * student logit is above -inf.  A logit of -inf has p = 0; q above 0 there makes the row's loss +inf. */

@@ -378,6 +378,20 @@ def test_sample_tokens_numbers_outside_their_range(ops, dev):
     ops.sample_tokens(logits[:0], u[:0], out[:0])
 
 
+@pytest.mark.parametrize("V", [9, 300, 5000])
+def test_sample_tokens_extreme_temperatures(ops, dev, V):
+    """Next to 0 only the largest logits are drawn, at infinity every finite one is alike."""
+    rng = np.random.default_rng(V)
+    logits = torch.from_numpy(rng.standard_normal((8, V)).astype(np.float32)).to(dev)
+    logits[1, 2] = logits[1, 5] = 50.0
+    logits[2, ::2] = -float("inf")
+    for T in (1e-310, 1e-40, 1e-5, 1e30, float("inf")):
+        for k, p in ((0, 1.0), (3, 1.0), (0, 0.5)):
+            check_sample(ops, dev, logits, rng.random(8) * 0.999, T, k, p, 0.0, some=0.3)
+    T = np.array([1e-45, 1e-38, 1.0, 1e38, np.inf, 0.0, 1e-3, 1e3])
+    check_sample(ops, dev, logits, rng.random(8) * 0.999, T, 4, 0.9, 0.0, some=0.3)
+
+
 @pytest.mark.parametrize("V", [48, 2000])
 def test_sample_tokens_follows_the_distribution(ops, dev, V):
     """Every token's borders: u on a fine grid visits the kept tokens in index order, each for its share of the grid (off by at

@@ -29,12 +29,12 @@ def sample(lib, rows=2, V=9, x=P, dtype=0, ld=9, T=1.0, k=0, p=1.0, m=0.0, u=P, 
 @pytest.mark.parametrize("call,bad", [
     (embed_fwd, dict(n=-1)), (embed_fwd, dict(D=0)), (embed_fwd, dict(V=-1)), (embed_fwd, dict(td=2)), (embed_fwd, dict(od=-1)), (embed_fwd, dict(ldt=7)),
     (embed_fwd, dict(ldo=0)), (embed_fwd, dict(stride=-1)), (embed_fwd, dict(tok=None)), (embed_fwd, dict(out=None)), (embed_fwd, dict(table=None)),
-    (embed_bwd, dict(n=1 << 31)), (embed_bwd, dict(V=(1 << 31) - 1)), (embed_bwd, dict(D=0)), (embed_bwd, dict(dd=3)), (embed_bwd, dict(ldd=0)),
+    (embed_bwd, dict(n=1 << 31)), (embed_fwd, dict(n=1 << 40)), (embed_bwd, dict(V=1 << 30, acc=0, wb=1 << 40)), (embed_bwd, dict(V=(1 << 31) - 1)), (embed_bwd, dict(D=0)), (embed_bwd, dict(dd=3)), (embed_bwd, dict(ldd=0)),
     (embed_bwd, dict(ldg=7)), (embed_bwd, dict(tok=None)), (embed_bwd, dict(dout=None)), (embed_bwd, dict(dt=None)), (embed_bwd, dict(ws=None)),
     (embed_bwd, dict(ws=P + 8)), (embed_bwd, dict(wb=64)),
     (distill, dict(rows=-1)), (distill, dict(V=0)), (distill, dict(K=0)), (distill, dict(K=1025, ldt=1025)), (distill, dict(dtype=5)), (distill, dict(ld=8)),
     (distill, dict(ldt=2)), (distill, dict(ldd=8)), (distill, dict(tau=0.0)), (distill, dict(tau=-1.0)), (distill, dict(tau=float("nan"))),
-    (distill, dict(tau=float("inf"))), (distill, dict(x=None)), (distill, dict(idx=None)), (distill, dict(val=None)), (distill, dict(loss=None)),
+    (distill, dict(tau=float("inf"))), (distill, dict(tau=1e-30)), (distill, dict(tau=1e30)), (distill, dict(x=None)), (distill, dict(idx=None)), (distill, dict(val=None)), (distill, dict(loss=None)),
     (distill, dict(d=P, ldd=12)),
     (sample, dict(rows=-1)), (sample, dict(V=0)), (sample, dict(dtype=2)), (sample, dict(ld=8)), (sample, dict(T=-0.5)), (sample, dict(T=float("nan"))),
     (sample, dict(k=-1)), (sample, dict(p=-0.1)), (sample, dict(p=float("nan"))), (sample, dict(m=-0.1)), (sample, dict(m=1.5)), (sample, dict(x=None)),

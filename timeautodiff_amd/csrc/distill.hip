@@ -295,14 +295,23 @@ int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
 extern "C" int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dtype, int64_t ld, const int64_t* index, const float* value,
                                 int64_t ld_t, float tau, const float* row_weight, float grad_scale, float* loss_rows, void* dlogits, int64_t ldd,
                                 tad_stream_t stream) {
-  TAD_CHECK(rows >= 0 && rows <= INT_MAX && V >= 1 && V <= INT_MAX && K >= 1 && K <= MAX_K, "tad_distill_loss: bad sizes (at most %d entries a row)", MAX_K);
+  TAD_CHECK(rows >= 0 && V >= 1 && V <= INT_MAX && K >= 1 && K <= MAX_K, "tad_distill_loss: bad sizes (at most %d entries a row)", MAX_K);
   TAD_CHECK(dtype == TAD_F32 || dtype == TAD_BF16, "tad_distill_loss: bad element type");
   TAD_CHECK(ld >= V && ld_t >= K && (!dlogits || ldd >= V), "tad_distill_loss: bad leading dimension");
-  TAD_CHECK(tau > 0.f && tau < INFINITY, "tad_distill_loss: the temperature has to be positive and finite");
+  TAD_CHECK(tau >= 1e-18f && tau <= 1e18f, "tad_distill_loss: the temperature has to lie between 1e-18 and 1e18");
   if (rows == 0) return TAD_OK;
   TAD_CHECK(logits && index && value && loss_rows, "tad_distill_loss: null pointer");
   TAD_CHECK(dlogits != logits || ldd == ld, "tad_distill_loss: a gradient in the logits' place needs their row stride");
-  const Args A = {rows, V, ld, ld_t, ldd, K, index, value, row_weight, (float)(1.4426950408889634074 / (double)tau), tau, grad_scale, loss_rows};
-  return dtype == TAD_F32 ? launch_distill<float>(A, (const float*)logits, (float*)dlogits, (hipStream_t)stream)
-                          : launch_distill<bf16_t>(A, (const bf16_t*)logits, (bf16_t*)dlogits, (hipStream_t)stream);
+  // at most 2^22 rows a launch: a grid holds fewer than 2^32 threads
+  const int64_t step = (int64_t)1 << 22;
+  for (int64_t r = 0; r < rows; r += step) {
+    const Args A = {rows - r < step ? rows - r : step, V, ld, ld_t, ldd, K, index + r * ld_t, value + r * ld_t, row_weight ? row_weight + r : nullptr,
+                    (float)(1.4426950408889634074 / (double)tau), tau, grad_scale, loss_rows + r};
+    const int64_t x = r * ld, d = r * ldd;
+    const int rc = dtype == TAD_F32
+                       ? launch_distill<float>(A, (const float*)logits + x, dlogits ? (float*)dlogits + d : nullptr, (hipStream_t)stream)
+                       : launch_distill<bf16_t>(A, (const bf16_t*)logits + x, dlogits ? (bf16_t*)dlogits + d : nullptr, (hipStream_t)stream);
+    if (rc != TAD_OK) return rc;
+  }
+  return TAD_OK;
 }

@@ -70,10 +70,11 @@ struct Settings {
   const int32_t* kr;
 };
 struct RowSettings {
-  double T, p, tmin;       // tmin: log2 of min_p
+  double T, c, p, tmin;    // c: log2(e) / T, finite (0 times it is 0); tmin: log2 of min_p
   int64_t k;
   __device__ RowSettings(const Settings& st, int64_t r) {
     T = st.Tr ? (double)st.Tr[r] : st.T;
+    c = fmin(1.4426950408889634074 / T, 1e300);
     k = st.kr ? (int64_t)st.kr[r] : st.k;
     p = st.pr ? (double)st.pr[r] : st.p;
     const double m = st.mr ? (double)st.mr[r] : st.minp;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
     if (lane == 0) out[r] = m == -INFINITY ? -1 : at;
     return;
   }
-  const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
+  const Scale sc = {m, rs.c, F};
   const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
   double w[E];
   uint32_t low = 0;                           // the ones below min_p
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     if (lo + lane + 64 * h < hi) held[h] = row.raw(lo + lane + 64 * h);
   // top-p alone: the sum of the weights too, roughly (each thread relative to its own largest)
   const bool guess = rs.T > 0.0 && !(rs.k > 0 && rs.k < V) && rs.p < 1.0 && V > CAP;
-  const float rough = (float)(1.4426950408889634074 / rs.T);
+  const float rough = (float)rs.c;
   float tm = -INFINITY, tz = 0.f;
   const auto look = [&](const float (&v)[VEC]) {
     float b = tm;
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   infinite = m == INFINITY;
   m = fminf(m, LARGEST);
   tm = fminf(tm, LARGEST);
-  const Scale sc = {m, 1.4426950408889634074 / rs.T, F};
+  const Scale sc = {m, rs.c, F};
   const bool by_k = rs.k > 0 && rs.k < V, by_p = rs.p < 1.0;
   // halves the distance between two keys: by value as long as that lies between them
   const auto between = [](uint32_t a, uint32_t b, int step) {
@@ -830,7 +831,7 @@ int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const
 extern "C" int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, int dtype, int64_t ld, double temperature, const float* temperature_rows,
                                  int64_t top_k, const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
                                  const float* min_p_rows, const float* u, int64_t* out, tad_stream_t stream) {
-  TAD_CHECK(rows >= 0 && rows <= INT_MAX && V >= 1 && V <= INT_MAX, "tad_sample_tokens: bad sizes");
+  TAD_CHECK(rows >= 0 && V >= 1 && V <= INT_MAX, "tad_sample_tokens: bad sizes");
   TAD_CHECK(dtype == TAD_F32 || dtype == TAD_BF16, "tad_sample_tokens: bad element type");
   TAD_CHECK(ld >= V, "tad_sample_tokens: bad leading dimension");
   TAD_CHECK(temperature_rows || temperature >= 0.0, "tad_sample_tokens: the temperature has to be 0 or more");
@@ -844,5 +845,15 @@ extern "C" int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, in
   const int whole = V <= 2048 ? 53 : 61, F = whole - lg < 44 ? whole - lg : 44;       // bits of the row's largest sum (a thread's: 53)
   const Settings st = {temperature, top_p, min_p, top_k, temperature_rows, top_p_rows, min_p_rows, top_k_rows};
   hipStream_t s = (hipStream_t)stream;
-  return dtype == TAD_F32 ? launch_sample<float>(rows, V, logits, ld, st, F, u, out, s) : launch_sample<bf16_t>(rows, V, logits, ld, st, F, u, out, s);
+  // at most 2^22 rows a launch: a grid holds fewer than 2^32 threads
+  const int64_t step = (int64_t)1 << 22;
+  for (int64_t r = 0; r < rows; r += step) {
+    const int64_t part = rows - r < step ? rows - r : step;
+    const Settings at = {st.T, st.p, st.minp, st.k, st.Tr ? st.Tr + r : nullptr, st.pr ? st.pr + r : nullptr, st.mr ? st.mr + r : nullptr,
+                         st.kr ? st.kr + r : nullptr};
+    const int rc = dtype == TAD_F32 ? launch_sample<float>(part, V, (const float*)logits + r * ld, ld, at, F, u + r, out + r, s)
+                                    : launch_sample<bf16_t>(part, V, (const bf16_t*)logits + r * ld, ld, at, F, u + r, out + r, s);
+    if (rc != TAD_OK) return rc;
+  }
+  return TAD_OK;
 }

@@ -517,7 +517,7 @@ int launch_fwd(int64_t n, int D, int64_t vocab, const int64_t* tok, int64_t tstr
   // four rows a lane where that still leaves every CU several waves
   const bool many = (cdiv64(n, 4) << ll) >= 256 * 1024;
   const int64_t grid = cdiv64(cdiv64(n, many ? 4 : 1) << ll, 256);
-  TAD_CHECK(grid <= INT_MAX, "tad_token_embed_fwd: too many tokens");
+  TAD_CHECK(grid < (1 << 24), "tad_token_embed_fwd: too many tokens");          // (a grid holds fewer than 2^32 threads)
 #define FWD_(VEC, U)                                                                                                                                   \
   hipLaunchKernelGGL((token_embed_fwd_kernel<TI, TO, VEC, U>), dim3((unsigned)grid), dim3(256), 0, s, n, nv, ll, vocab, tok, tstride, scale, (const TI*)table, \
                      ldt, (TO*)out, ldo)
@@ -593,7 +593,8 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
   const int64_t kb = key_bytes(n);
   TAD_CHECK(workspace && aligned16(workspace) && workspace_bytes >= 2 * kb + COUNT_BYTES + 2 * g.nchunks * D * 4,
             "tad_token_embed_bwd: workspace of %lld bytes, 16-byte aligned, needed", (long long)tad_token_embed_bwd_workspace_bytes(n, D));
-  TAD_CHECK(g.nchunks * g.ctiles + cdiv64(vocab, ZROWS * GW) < INT_MAX && g.nchunks * cdiv64(D, 64) < INT_MAX, "tad_token_embed_bwd: too many tokens");
+  TAD_CHECK(g.nchunks * g.ctiles + cdiv64(vocab, ZROWS * GW) < (1 << 23) && g.nchunks * cdiv64(D, wide ? 256 : 64) < (1 << 24),
+            "tad_token_embed_bwd: too many tokens or rows");                        // (a grid holds fewer than 2^32 threads)
   // the direct form, where its workgroups are few (2048: two rounds of the chip), read the tokens few times (2^22: 32 MB from L2)
   // and a row of the table does not get so many tokens that the one workgroup's time is theirs (2400 tokens of 128 columns
   // into 50, 500, 1700 rows: 11 us against 15 sorted; 4096 into 2 rows: 24 against 17; 100 into 40000 rows: 99 against 15)
@@ -651,6 +652,5 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
                          a, part, dtable, ld_dtable);
     TAD_LAUNCH_CHECK();
   }
-  tad_note_kernel("embed_grad_sum_kernel");
   return TAD_OK;
 }

@@ -1013,8 +1013,8 @@ def token_embed_bwd(tokens, dout, dtable, scale=1.0, accumulate=True, workspace=
 def distill_loss(logits, index, value, loss_rows, temperature=1.0, row_weight=None, grad_scale=1.0, dlogits=None):
     """Distillation from a teacher's top logits: loss_rows[r] = w_r tau^2 KL(q || p), q the softmax of value[r] / tau over the
     entries whose index lies in [0, V), p the softmax of logits[r] / tau; dlogits (optional; may be logits itself) =
-    grad_scale * the gradient.  logits / dlogits [..., V] float32 or bfloat16, index int64 and value float32 [..., K],
-    row_weight and loss_rows contiguous float32 of one number per row."""
+    grad_scale * the gradient.  logits / dlogits [..., V] float32 or bfloat16, index int64 and value float32 [..., K] of one
+    row stride, row_weight and loss_rows contiguous float32 of one number per row."""
     dev = torch.cuda.current_device()
     xp, rows, V, ld = _rows(logits, dev)
     ip, ri, K, ldi = _rows(index, dev)
