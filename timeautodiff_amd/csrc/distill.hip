@@ -35,11 +35,6 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 // columns through LDS, which only the row's own lanes touch: its order within the wave is all the synchronisation.  An index
 // that comes twice is seen by the entry whose mark at the column was overwritten; such entries add up all q of the index in
 // order and write the same sum.
-__device__ __forceinline__ void lds_in_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* logits, T* dlogits) {
   constexpr int R = 256 / G;                          // rows of a workgroup
@@ -160,7 +155,13 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
   const int64_t r = blockIdx.x, V = A.V;
   const T* x = logits + r * A.ld;
   T* d = dlogits ? dlogits + r * A.ldd : nullptr;
-  const RowPieces<T> row(x, V);
+  // `head` elements up to a 16-byte boundary, np whole pieces from there, and what is left: head and rest one by one, by the
+  // first threads.  (The gradient's rows may lie differently: its stores need the alignment of an element only.)
+  const int head = (int)(-((uintptr_t)x / sizeof(T)) & (VEC - 1));
+  const int64_t np = (V - head) / VEC;
+  const int edge = (int)(V - np * VEC);
+  const int64_t at_edge = tid < head ? tid : V - edge + tid;
+  const auto piece = [&](int64_t i) { return *reinterpret_cast<const pack*>(x + head + i * VEC); };
   const float w = A.weight ? A.weight[r] : 1.f;
   float m = LOWEST, z = 0.f, tm = LOWEST, tz = 0.f;
   // the entries and the student's logits at them, asked for before anything waits
@@ -189,15 +190,22 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
     z = s;
   };
   pack held[H];
+  float last = -INFINITY;
   if (w != 0.f) {
 #pragma unroll
     for (int k = 0; k < H; ++k)
-      if (tid + k * NT < row.np) held[k] = row.raw(tid + k * NT);
+      if (tid + k * NT < np) held[k] = piece(tid + k * NT);
+    if (tid < edge) last = (float)x[at_edge];
 #pragma unroll
     for (int k = 0; k < H; ++k)
-      if (tid + k * NT < row.np) add(held[k]);
+      if (tid + k * NT < np) add(held[k]);
 #pragma unroll 4
-    for (int64_t i = tid + H * NT; i < row.np; i += NT) add(row.raw(i));
+    for (int64_t i = tid + H * NT; i < np; i += NT) add(piece(i));
+    if (tid < edge) {
+      const float b = fmaxf(m, last);
+      z = z * ex2((m - b) * A.c) + ex2((last - b) * A.c);
+      m = b;
+    }
   }
 #pragma unroll
   for (int n = 0; n < KE; ++n)
@@ -235,25 +243,18 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
   if (tid == 0) A.loss[r] = w * A.tau * A.tau * (l * LN2);
   if (!d) return;
   const float gz = g * iz;
-  const bool together = (((uintptr_t)d ^ (uintptr_t)x) & 15) == 0;
   const auto put = [&](int64_t i, const pack& p) {
     pack o;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = (T)(gz * ex2(((float)p[e] - m) * A.c));
-    const int64_t j = row.first(i);
-    if (together && j >= 0 && j + VEC <= V) {
-      __builtin_nontemporal_store(o, reinterpret_cast<pack*>(d + j));
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (j + e >= 0 && j + e < V) d[j + e] = o[e];
-    }
+    __builtin_nontemporal_store(o, reinterpret_cast<pack*>(d + head + i * VEC));
   };
 #pragma unroll 4
-  for (int64_t i = tid < row.np ? (row.np - 1 - tid) / NT * NT + tid : -1; i >= H * NT; i -= NT) put(i, row.raw(i));
+  for (int64_t i = tid < np ? (np - 1 - tid) / NT * NT + tid : -1; i >= H * NT; i -= NT) put(i, piece(i));
 #pragma unroll
   for (int k = 0; k < H; ++k)
-    if (tid + k * NT < row.np) put(tid + k * NT, held[k]);
+    if (tid + k * NT < np) put(tid + k * NT, held[k]);
+  if (tid < edge) d[at_edge] = (T)(gz * ex2((last - m) * A.c));
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < KE; ++n) {

@@ -57,3 +57,10 @@ __device__ __forceinline__ V lanes_before(V v, int lane) {
   }
   return inc - v;
 }
+
+// LDS accesses of a wave before and after this are in order for its own lanes (the hardware keeps a wave's LDS order; this keeps
+// the compiler to it)
+__device__ __forceinline__ void lds_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}

@@ -234,6 +234,8 @@ struct RowState {
     Candidate pair[PAIRS];
   };
   uint32_t cnt[BINS];
+  uint32_t piece[NW][64];
+  u64 reach[2][NW];
   u64 wsum[NW];
   uint32_t wcnt[NW];
   float wmax[NW], wmin[NW];
@@ -273,19 +275,34 @@ __device__ __forceinline__ I block_scan(I v, I* s, I* sum) {
   return before + inc - v;
 }
 
-// sorts list[0 .. P), P a power of two: falling, or rising
+// sorts list[0 .. P), P a power of two: falling, or rising.  Up to WAVE_SORT a single wave does it, without barriers (256: 36
+// steps of about 0.06 us, where a barrier of 16 waves alone takes four times that)
+constexpr int WAVE_SORT = 512;
 template <int NT>
 __device__ void sort_list(u64* list, int P, bool falling) {
+  const auto step = [&](int size, int stride, int from, int by) {
+    for (int i = from; i < P / 2; i += by) {
+      const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+      const u64 a = list[lo], b = list[hi];
+      if ((a < b) == (((lo & size) == 0) == falling) && a != b) { list[lo] = b; list[hi] = a; }
+    }
+  };
+  __syncthreads();
+  if (P <= WAVE_SORT) {
+    if (threadIdx.x < 64)
+      for (int size = 2; size <= P; size <<= 1)
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+          step(size, stride, threadIdx.x, 64);
+          lds_in_order();
+        }
+    __syncthreads();
+    return;
+  }
   for (int size = 2; size <= P; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      step(size, stride, threadIdx.x, NT);
       __syncthreads();
-      for (int i = threadIdx.x; i < P / 2; i += NT) {
-        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-        const u64 a = list[lo], b = list[hi];
-        if ((a < b) == (((lo & size) == 0) == falling) && a != b) { list[lo] = b; list[hi] = a; }
-      }
     }
-  __syncthreads();
 }
 __device__ __forceinline__ int pow2_at_least(int n) {
   int P = 64;
@@ -309,7 +326,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   bool infinite = false;                    // +inf among the logits
 
   // every piece of the share, and every element of the piece (v[e])
-#define EACH_PIECE(...) _Pragma("unroll 4") ONE_BY_ONE(__VA_ARGS__)
+#define EACH_PIECE(...) _Pragma("unroll 2") ONE_BY_ONE(__VA_ARGS__)
 #define ONE_BY_ONE(...)                                                                  \
   for (int64_t i = lo + lane; i < hi; i += 64) {                                         \
     float v[VEC];                                                                        \
@@ -321,13 +338,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   }
 #define EACH(...) _Pragma("unroll") for (int e = 0; e < VEC; ++e) { __VA_ARGS__ }
 
-  // the thread's largest logit, the row's, and the smallest of the threads'; the thread's first H pieces stay in registers
-  // for the next look at the row
-  constexpr int H = 16;
-  typename RowPieces<T>::pack held[H];
-#pragma unroll
-  for (int h = 0; h < H; ++h)
-    if (lo + lane + 64 * h < hi) held[h] = row.raw(lo + lane + 64 * h);
+  // the thread's largest logit, the row's, and the smallest of the threads'
   // top-p alone: the sum of the weights too, roughly (each thread relative to its own largest)
   const bool guess = rs.T > 0.0 && !(rs.k > 0 && rs.k < V) && rs.p < 1.0 && V > CAP;
   const float rough = (float)rs.c;
@@ -342,37 +353,49 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     }
     tm = b;
   };
+  // (the largest of each of the thread's first H pieces stays in a register: which pieces a later look at the row needs)
+  constexpr int H = 16;
+  float most[H];
 #pragma unroll
-  for (int h = 0; h < H; ++h)
-    if (lo + lane + 64 * h < hi) {
+  for (int h = 0; h < H; ++h) {
+    const int64_t i = lo + lane + 64 * h;
+    most[h] = -INFINITY;
+    if (i < hi) {
       float v[VEC];
-      EACH(v[e] = (float)held[h][e];)
+      row.load(i, v);
       look(v);
+      EACH(most[h] = fmaxf(most[h], v[e]);)
     }
+  }
   for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
     float v[VEC];
     row.load(i, v);
     look(v);
   }
-  // the pieces of which an element reaches f: `body` of every element (a logit, its index) of them that does
-  const auto each_from = [&](float f, const auto& body) {
-    const auto one = [&](int64_t i, const float (&v)[VEC]) {
-      float b = -INFINITY;
-      EACH(b = fmaxf(b, v[e]);)
-      if (b >= f) EACH(if (v[e] >= f) body(infinite && v[e] == INFINITY ? LARGEST : v[e], row.first(i) + e);)
+  // The wave's pieces with an element that reaches f: S.piece[wave] has them, up to 64; returns how many there are.
+  const auto pieces_from = [&](float f) {
+    int n = 0;
+    const auto take = [&](bool in, int64_t i) {
+      const u64 b = __ballot(in);
+      const int at = n + __popcll(b & ((1ull << lane) - 1));
+      if (in && at < 64) S.piece[wave][at] = (uint32_t)i;
+      n += __popcll(b);
     };
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-      if (lo + lane + 64 * h < hi) {
-        float v[VEC];
-        EACH(v[e] = (float)held[h][e];)
-        one(lo + lane + 64 * h, v);
-      }
-    for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
-      float v[VEC];
-      row.load(i, v);
-      one(i, v);
+    for (int h = 0; h < H; ++h) {
+      if (lo + 64 * h >= hi) break;
+      take(most[h] >= f, lo + lane + 64 * h);
     }
+    for (int64_t i0 = lo + 64 * H; i0 < hi; i0 += 64) {
+      float v[VEC], b = -INFINITY;
+      if (i0 + lane < hi) {
+        row.load(i0 + lane, v);
+        EACH(b = fmaxf(b, v[e]);)
+      }
+      take(b >= f, i0 + lane);
+    }
+    lds_in_order();
+    return n;
   };
   float m = across<64, Max>(tm), least = across<64, Min>(tm > -INFINITY ? tm : INFINITY);
   if (lane == 0) {
@@ -391,8 +414,13 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     return;
   }
   if (!(rs.T > 0.0)) {
-    u64 at = ~0ull;                         // the lowest index of the largest
-    each_from(m, [&](float, int64_t j) { at = (u64)j < at ? (u64)j : at; });
+    u64 at = ~0ull;                         // the lowest index of the largest (pieces come in order: the first that has it)
+    if (pieces_from(m) > 0) {
+      const int64_t i = S.piece[wave][0];
+      float v[VEC];
+      row.load(i, v);
+      EACH(if (v[VEC - 1 - e] == m) at = (u64)(row.first(i) + VEC - 1 - e);)
+    }
     at = across<64, Min>(at);
     if (lane == 0) S.wsum[wave] = at;
     __syncthreads();
@@ -417,21 +445,54 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   if ((by_k && rs.k <= CAP / 2 && rs.k <= NT) || ((by_k || by_p) && V <= CAP) || guess) {
     const int64_t kk = by_k ? rs.k : guess ? GUESS : V;
     // where kk threads' largest reach `floor`, at least kk logits do; not many more than kk are wanted
+    // (the numbers of three values at a time, one barrier a step)
     float floor = -LARGEST;
-    if (V > CAP && __syncthreads_count(tm >= least) >= kk) {
+    int step = 0;
+    const auto reach = [&](float f1, float f2, float f3) {        // 16 bits each
+      const u64 mine = (u64)__popcll(__ballot(tm >= f1)) | (u64)__popcll(__ballot(tm >= f2)) << 16 | (u64)__popcll(__ballot(tm >= f3)) << 32;
+      if (lane == 0) S.reach[step & 1][wave] = mine;
+      __syncthreads();
+      u64 all = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) all += S.reach[step & 1][w];
+      ++step;
+      return all;
+    };
+    if (V > CAP && (int64_t)(reach(least, least, least) & 0xffff) >= kk) {
       uint32_t a = key_of(least), b = key_of(m);
-      for (int step = 0; step < 24 && a < b; ++step) {
-        const uint32_t k = between(a, b, step);
-        const int n = __syncthreads_count(tm >= logit_of(k));
-        if (n >= kk) a = k; else b = k - 1;
-        if (n >= kk && n <= kk + kk / 4 + 8) break;
+      while (a < b && step < 16) {
+        const uint32_t k2 = between(a, b, step), k1 = between(a, k2, step), k3 = between(k2, b, step);
+        const u64 all = reach(logit_of(k1), logit_of(k2), logit_of(k3));
+        const int n1 = (int)(all & 0xffff), n2 = (int)(all >> 16 & 0xffff), n3 = (int)(all >> 32);
+        int n = 0;
+        if (n3 >= kk) { a = k3; n = n3; }
+        else if (n2 >= kk) { a = k2; b = k3 - 1; n = n2; }
+        else if (n1 >= kk) { a = k1; b = k2 - 1; n = n1; }
+        else b = k1 - 1;
+        if (n && n <= kk + kk / 4 + 8) break;
       }
       floor = logit_of(a);
     }
-    each_from(floor, [&](float l, int64_t j) {
-      const uint32_t at = atomicAdd(&S.n, 1u);
-      if (at < CAP) S.list[at] = (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)j;
-    });
+    // every lane takes one of the wave's pieces that reach it
+    {
+      const int np = pieces_from(floor);
+      const bool on = lane < np && np <= 64;
+      const int64_t i = on ? S.piece[wave][lane] : 0;
+      float v[VEC];
+      int n = 0;
+      if (on) {
+        row.load(i, v);
+        EACH(v[e] = infinite && v[e] == INFINITY ? LARGEST : v[e]; n += v[e] >= floor;)
+      }
+      int at = lanes_before<64>(n, lane);
+      int base = 0;
+      if (lane == 63) base = (int)atomicAdd(&S.n, (uint32_t)(np <= 64 ? at + n : CAP + 1));
+      at += __builtin_amdgcn_readlane(base, 63);
+      if (on) EACH(if (v[e] >= floor) {
+        if (at < CAP) S.list[at] = (u64)key_of(v[e]) << 32 | (uint32_t)~(uint32_t)(row.first(i) + e);
+        ++at;
+      })
+    }
     __syncthreads();
     int n = S.n < CAP + 1 ? (int)S.n : CAP + 1;
     const int nk = kk < n && !guess ? (int)kk : n;
@@ -656,7 +717,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       if (lane == 0) S.wsum[wave] = w;
       __syncthreads();
       for (int i = tid; i <= (int)S.at; i += NT) {
-        const int64_t piece = ((int64_t)(uint32_t)~(uint32_t)S.list[i] + row.a) / VEC;
+        const int64_t piece = (int64_t)(uint32_t)~(uint32_t)S.list[i] / VEC;
         atomicAdd(&S.wsum[piece / seg], whole_number(weight_of(sc, logit_of((uint32_t)(S.list[i] >> 32)))));
       }
     }
@@ -703,68 +764,15 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     }
   }
 
-  // ---- by index: the waves' masses, then the share in which the sum passes divided among the waves, until a wave holds it
-  const bool everything = cut == -LARGEST && rs.tmin == -INFINITY;
-  // the kept weights of a piece; tie: ties before it
-  const auto kept = [&](const float (&v)[VEC], uint32_t tie, double (&w)[VEC]) {
-    double sum = 0;
-    if (everything) {
-      EACH(w[e] = weight_of(sc, v[e]); sum += w[e];)
-    } else if (ties == ALL) {
-      EACH(const double t = log2_weight(sc, v[e]); w[e] = v[e] >= cut && t >= rs.tmin ? fixed_weight(sc, t) : 0.0; sum += w[e];)
-    } else {
-      EACH(const double t = log2_weight(sc, v[e]); const bool in = (v[e] > cut || (v[e] == cut && tie++ < ties)) && t >= rs.tmin;
-           w[e] = in ? fixed_weight(sc, t) : 0.0; sum += w[e];)
-    }
-    return sum;
-  };
-  int64_t A = 0, B = row.np;
+  // ---- by index: the waves' masses, then the share in which the sum passes divided among the waves element by element, until
+  // the lanes of a wave hold it
+  const int64_t width = seg * VEC;           // elements of a wave's share
+  int64_t A = 0, B = V;
   u64 base = 0, target = 0;
-  uint32_t tie = 0;                          // ties before piece A
-  for (bool first = true; first || B - A > 64; first = false) {
-    const int64_t share = (B - A + NW - 1) / NW, a = A + wave * share < B ? A + wave * share : B, b = a + share < B ? a + share : B;
-    uint32_t eq = 0;
-    __syncthreads();
-    if (ties != ALL) {
-      for (int64_t i = a + lane; i < b; i += 64) {
-        float v[VEC];
-        row.load(i, v);
-        EACH(eq += (infinite && v[e] == INFINITY ? LARGEST : v[e]) == cut;)
-      }
-      eq = across<64, Add>(eq);
-      if (lane == 0) S.wcnt[wave] = eq;
-      __syncthreads();
-      eq = tie;
-      for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
-    }
-    if (!(first && shares)) {
-      double mass = 0;
-      for (int64_t i0 = a; i0 < b; i0 += 64) {
-        float v[VEC], most = -INFINITY;
-        double w[VEC];
-        if (i0 + lane < b) row.load(i0 + lane, v);
-        else EACH(v[e] = -INFINITY;)
-        if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
-        EACH(most = fmaxf(most, v[e]);)
-        if (!__any(most >= cut)) continue;
-        uint32_t before = 0;
-        if (ties != ALL) {
-          uint32_t n = 0;
-          EACH(n += v[e] == cut;)
-          before = eq + lanes_before<64>(n, lane);
-          eq += across<64, Add>(n);
-        }
-        mass += kept(v, before, w);
-      }
-      const u64 all = across<64, Add>((u64)mass);
-      if (lane == 0) S.wsum[wave] = all;
-      __syncthreads();
-    }
-    if (first) {
-      u64 all = 0;
-      for (int w = 0; w < NW; ++w) all += S.wsum[w];
-      target = target_of(uu, all);
-    }
+  uint32_t tie = 0;                          // ties before A
+  const auto clean = [&](float l) { return infinite && l == INFINITY ? LARGEST : l; };
+  // the share in which the sum passes (S.wsum: masses, S.wcnt: ties)
+  const auto choose = [&](int64_t share) {
     int w = 0;
     for (; w < NW - 1 && base + S.wsum[w] <= target; ++w) {
       base += S.wsum[w];
@@ -772,22 +780,82 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     }
     A += w * share;
     B = A + share < B ? A + share : B;
+  };
+  uint32_t eq = 0;
+  __syncthreads();
+  if (ties != ALL) {
+    ONE_BY_ONE(EACH(eq += v[e] == cut;))
+    eq = across<64, Add>(eq);
+    if (lane == 0) S.wcnt[wave] = eq;
+    __syncthreads();
+    eq = 0;
+    for (int w = 0; w < wave; ++w) eq += S.wcnt[w];
+  }
+  if (!shares) {
+    double mass = 0;
+    if (cut == -LARGEST && rs.tmin == -INFINITY) {
+      ONE_BY_ONE(EACH(mass += weight_of(sc, v[e]);))
+    } else if (ties == ALL) {
+      ONE_BY_ONE(float b = -INFINITY; EACH(b = fmaxf(b, v[e]);) if (__any(b >= cut))
+                     EACH(const double t = log2_weight(sc, v[e]); mass = add_if(v[e] >= cut && t >= rs.tmin, fixed_weight(sc, t), mass);))
+    } else {
+      for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+        float v[VEC];
+        if (i0 + lane < hi) row.load(i0 + lane, v);
+        else EACH(v[e] = -INFINITY;)
+        uint32_t n = 0;
+        EACH(v[e] = clean(v[e]); n += v[e] == cut;)
+        uint32_t before = eq + lanes_before<64>(n, lane);
+        eq += across<64, Add>(n);
+        EACH(const double t = log2_weight(sc, v[e]); const bool in = (v[e] > cut || (v[e] == cut && before++ < ties)) && t >= rs.tmin;
+             mass = add_if(in, fixed_weight(sc, t), mass);)
+      }
+    }
+    const u64 all = across<64, Add>((u64)mass);
+    if (lane == 0) S.wsum[wave] = all;
+    __syncthreads();
+  }
+  {
+    u64 all = 0;
+    for (int w = 0; w < NW; ++w) all += S.wsum[w];
+    target = target_of(uu, all);
+  }
+  choose(width);
+  // a lane's element of 64 neighbours from j0 on: its kept weight; ties: before j0, moved on
+  const auto kept = [&](int64_t j0, int64_t end, uint32_t& before) {
+    const float l = j0 + lane < end ? clean((float)row.x[j0 + lane]) : -INFINITY;
+    const double t = log2_weight(sc, l);
+    bool in = l >= cut && t >= rs.tmin;
+    if (ties != ALL) {
+      const u64 b = __ballot(l == cut);
+      in = in && (l > cut || before + __popcll(b & ((1ull << lane) - 1)) < ties);
+      before += __popcll(b);
+    }
+    return in ? fixed_weight(sc, t) : 0.0;
+  };
+  while (B - A > 64) {
+    const int64_t share = ((B - A + NW - 1) / NW + 63) / 64 * 64, a = A + wave * share < B ? A + wave * share : B, b = a + share < B ? a + share : B;
+    uint32_t before = tie;
+    __syncthreads();
+    if (ties != ALL) {
+      uint32_t n = 0;
+      for (int64_t j = a + lane; j < b; j += 64) n += clean((float)row.x[j]) == cut;
+      n = across<64, Add>(n);
+      if (lane == 0) S.wcnt[wave] = n;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) before += S.wcnt[w];
+    }
+    double mass = 0;
+#pragma unroll 1
+    for (int64_t j0 = a; j0 < b; j0 += 64) mass += kept(j0, b, before);
+    const u64 all = across<64, Add>((u64)mass);
+    if (lane == 0) S.wsum[wave] = all;
+    __syncthreads();
+    choose(share);
   }
   if (wave != 0) return;
-  float v[VEC];
-  double w[VEC];
-  if (A + lane < B) row.load(A + lane, v);
-  else EACH(v[e] = -INFINITY;)
-  if (infinite) EACH(v[e] = v[e] == INFINITY ? LARGEST : v[e];)
-  uint32_t n = 0;
-  EACH(n += v[e] == cut;)
-  const u64 sum = (u64)kept(v, tie + lanes_before<64>(n, lane), w);
-  u64 before = base + lanes_before<64>(sum, lane);
-  if (before <= target && target < before + sum) {
-    int at = 0;
-    EACH(before += (u64)w[e]; at += before <= target;)
-    out[r] = row.first(A + lane) + at;
-  }
+  const u64 w = (u64)kept(A, B, tie), before = base + lanes_before<64>(w, lane);
+  if (before <= target && target < before + w) out[r] = A + lane;
 #undef EACH_PIECE
 #undef ONE_BY_ONE
 #undef EACH

@@ -146,7 +146,7 @@ __global__ __launch_bounds__(1024) void sort_rank_kernel(int n, int64_t vocab, c
 // wave a contiguous share of it, so that keys of one digit keep their order: the first launch counts digits by tile, the
 // second adds up what comes before (lower digits; earlier tiles; earlier waves) and moves the keys.  No workgroup waits for
 // another, and no distribution of tokens is worse than another.
-constexpr int MAX_BINS = 512, MAX_TILES = 64, RWAVES = 8;
+constexpr int MAX_BINS = 512, MAX_TILES = 128, RWAVES = 8;
 
 struct Digit {
   const int64_t* tok;       // the first digit's source
