@@ -284,7 +284,7 @@ int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
   else if (A.V <= 1024) SHORT_(64, 16);
   else if (A.V <= 16384) ROW_(256, 4);
   else if (A.V <= (sizeof(T) == 2 ? 65536 : 16384)) ROW_(512, 8);
-  else ROW_(512, 20);
+  else ROW_(512, 16);
 #undef SHORT_
 #undef ROW_
   TAD_LAUNCH_CHECK();
