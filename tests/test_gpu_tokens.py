@@ -606,3 +606,23 @@ def test_sample_tokens_of_peaked_rows(ops, dev, V):
     for dtype in (torch.float32, torch.bfloat16):
         for s in SETTINGS:
             check_sample(ops, dev, torch.from_numpy(x).to(dev, dtype), rng.random(rows) * 0.999, *s, some=0.8)
+
+
+def test_token_ops_are_traced_with_their_costs(ops, dev):
+    """An installed LaunchTrace sees every call with its bytes: each operand and result once."""
+    tok, table, out = torch.randint(0, 5, (30,), device=dev), torch.randn(5, 8, device=dev), torch.empty(30, 8, device=dev)
+    logits, u, code = torch.randn(6, 40, device=dev), torch.rand(6, device=dev), torch.empty(6, dtype=torch.int64, device=dev)
+    index, value, loss = torch.randint(0, 40, (6, 3), device=dev), torch.randn(6, 3, device=dev), torch.empty(6, device=dev)
+    with ops.LaunchTrace() as tr:
+        ops.token_embed_fwd(tok, table, out)
+        ops.token_embed_bwd(tok, out, table)
+        ops.token_embed_bwd(tok, out, table, accumulate=False)
+        ops.distill_loss(logits, index, value, loss)
+        ops.distill_loss(logits, index, value, loss, dlogits=logits)
+        ops.sample_tokens(logits, u, code)
+    seen = {}
+    for key, (calls, ms, flops, nbytes, issued) in tr.summary().items():
+        seen.setdefault(key[0], []).append((calls, nbytes))
+    assert seen["tad_token_embed_fwd"] == [(1, 30 * 8 + 5 * 32 + 30 * 32)]
+    assert sum(c for c, _ in seen["tad_token_embed_bwd"]) == 2 and sum(c for c, _ in seen["tad_distill_loss"]) == 2
+    assert seen["tad_sample_tokens"] == [(1, 6 * (160 + 12))]

@@ -34,7 +34,8 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 // The row stays in registers (E logits a lane), statistics go across the G lanes by DPP, and the teacher's q reach their
 // columns through LDS, which only the row's own lanes touch: its order within the wave is all the synchronisation.  An index
 // that comes twice is seen by the entry whose mark at the column was overwritten; such entries add up all q of the index in
-// order and write the same sum.
+// order and write the same sum.  98304 x 48 float32, 8 entries: 11.3 us, 4.2 TB/s, and about as much instructions as HBM (q by
+// 64-bit integer atomics and reductions by lane shuffles: 17 us).
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* logits, T* dlogits) {
   constexpr int R = 256 / G;                          // rows of a workgroup
@@ -122,8 +123,11 @@ __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* log
 }
 
 // ---------------------------------------------------------------- long rows: a workgroup per row
-// Two passes over the row: maximum and sum in one (every thread rescales its sum when its maximum grows), then the gradient,
-// from the row's end backwards, where the caches still hold it.
+// Two passes over the row: maximum and sum in one (every thread rescales its sum when its maximum grows), then the gradient.
+// A thread's first H pieces of 16 bytes stay in registers in between; the others are read again from the row's end backwards,
+// where the caches still hold it, and the gradient goes past the caches.  4096 x 131072 bf16: 410 us, 4.9 TB/s of what it
+// moves (nothing held 516, H = 8 / 16 / 20: 452 / 422 / 445, 24 at one workgroup a CU: 455; 1024 threads: 439; stores
+// through the caches: 569); 512 x 32001 float32, the loss alone: 12.3 us, 4.8 TB/s.
 template <int NW, bool MAX>
 __device__ __forceinline__ void block_two(float& a, float& b, float (*s)[NW]) {      // largest, or sum, of two values at once
   a = MAX ? across<64, Max>(a) : wave_sum(a);
@@ -272,6 +276,10 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
 
 template <typename T>
 int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
+  // 4, 16 or 64 lanes a row, so that a lane has at most 16 logits; then, by the row's bytes, workgroups of 256 threads that hold
+  // it whole (16384 x 5000 bf16: 103 us; 512 threads: 119) or of 512: with 8 pieces a thread held up to 16 of them in all (65536
+  // bf16: 222 us against 236 with 24) or in float32, whose pieces are fewer logits, up to 8, beyond with 16 (4096 x 32001: 217
+  // against 259 with 8)
 #define SHORT_(G, E) hipLaunchKernelGGL((distill_short_kernel<T, G, E>), dim3((unsigned)cdiv64(A.rows, 256 / G)), dim3(256), 0, s, A, x, d)
 #define ROW_(NT, H) hipLaunchKernelGGL((distill_row_kernel<T, NT, H>), dim3((unsigned)A.rows), dim3(NT), 0, s, A, x, d)
   if (A.V <= 16) SHORT_(4, 4);

@@ -63,7 +63,8 @@ __device__ __forceinline__ void stream_pack(float* p, const float (&v)[VEC]) {
 
 // ---------------------------------------------------------------- forward
 // L lanes (a power of two, at most a wave) walk the columns of one row; a wave holds 64 / L rows side by side and U of them one
-// after another, whose loads are all issued before the first is used.
+// after another, whose loads are all issued before the first is used.  32768 x 2048 bf16: 49 us, 5.5 TB/s; 98304 x 128 float32
+// to bf16: 8.5 us, 3.1 TB/s (its waves wait once for a token and once for a row).
 template <typename TI, typename TO, int VEC, int U>
 __global__ __launch_bounds__(256) void token_embed_fwd_kernel(int64_t n, int nv, int lanes_log2, int64_t vocab, const int64_t* __restrict__ tok,
                                                               int64_t tstride, float scale, const TI* __restrict__ table, int64_t ldt,
@@ -106,7 +107,8 @@ __device__ __forceinline__ u64 key_at(const int64_t* tok, int64_t tstride, int64
 }
 
 // Up to RANK_N tokens: every token's place is counted directly, all pairs compared: a workgroup holds all tokens in LDS and
-// counts for 64 of them, each of its 16 waves over a sixteenth of the others (two instructions a comparison of 64 lanes).
+// counts for 64 of them, each of its 16 waves over a sixteenth of the others (two instructions a comparison of 64 lanes).  2400
+// tokens: 6.7 us, most of it the wait for the tokens (a bitonic sort of them in one workgroup: 35).
 constexpr int RANK_N = 8192;
 __global__ __launch_bounds__(1024) void sort_rank_kernel(int n, int64_t vocab, const int64_t* __restrict__ tok, int64_t tstride, u64* __restrict__ keys) {
   __shared__ __attribute__((aligned(16))) uint32_t s[RANK_N];
@@ -145,7 +147,8 @@ __global__ __launch_bounds__(1024) void sort_rank_kernel(int n, int64_t vocab, c
 // More: by digits of up to 9 bits from the lowest, two launches a digit.  A workgroup has a tile of neighbouring keys, every
 // wave a contiguous share of it, so that keys of one digit keep their order: the first launch counts digits by tile, the
 // second adds up what comes before (lower digits; earlier tiles; earlier waves) and moves the keys.  No workgroup waits for
-// another, and no distribution of tokens is worse than another.
+// another, and no distribution of tokens is worse than another.  98304 tokens of 9 bits: 3.2 + 9.5 us, latency of 48 to 96
+// workgroups (tiles of a quarter to a half of that number are slower, more of them read more counts).
 constexpr int MAX_BINS = 512, MAX_TILES = 128, RWAVES = 8;
 
 struct Digit {
@@ -244,6 +247,8 @@ __global__ __launch_bounds__(512) void sort_move_kernel(Digit d, int tiles, cons
 // A run of equal tokens inside a wave's share is a finished row of dtable.  What reaches over an edge between waves of the
 // workgroup is added up in LDS, what reaches over its edges goes to the workspace (slot 0: the run that came in from the
 // left; slot 1: one that begins here and goes on) and is added up by the launch behind, always in the order of positions.
+// Eight rows are in flight a wave.  32768 x 2048 bf16 into 65536 rows, zeros included: 140 us, 4.8 TB/s; 98304 x 128 float32 into
+// 500: 11.6 us, 4.4 TB/s.
 constexpr int GW = 8;
 constexpr int ZROWS = 8;      // rows of the table a wave of the zero part looks after
 
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
 }
 
 // Runs that reach over the edges of chunks: a workgroup for each chunk in which one begins (the others leave at once) and
-// each 64 * VEC columns; its waves add every fourth part, and the four sums are added in order.
+// each 64 * VEC columns; its waves add every fourth part, and the four sums are added in order.  5 us where most leave.
 template <int VEC>
 __global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, int64_t vocab, int P, int64_t nchunks, int ctiles, float scale,
                                                               int accumulate, const u64* __restrict__ keys, const float* __restrict__ part,
@@ -428,7 +433,8 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, 
 }
 
 // Few tokens and few rows: a workgroup for each row of the table and each 64 * VEC columns looks through all tokens itself, each
-// of its 16 waves through a sixteenth of them, and adds what it finds: one launch, where sorting takes three.
+// of its 16 waves through a sixteenth of them, and adds what it finds: one launch, where sorting takes three.  2400 x 128 into 50
+// rows: 6.8 us (sorted: 15).
 constexpr int DIRECT_N = 4096, DIRECT_WAVES = 16;
 
 template <typename T, int VEC>
