@@ -593,6 +593,22 @@ def test_sample_tokens_very_long_rows(ops, dev, V):
             check_sample(ops, dev, logits, u, T, k, p, m, some=0.6)
 
 
+# a list of candidates holds few of them; its length, and whether each is compared with each, hang on top-k, the row and the rows
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,tops", [(3, 2500, (111, 112, 113, 160, 224, 225, 448)), (260, 2500, (112, 113, 160, 161, 225)),
+                                         (2, 30000, (224, 225, 320, 321, 448)), (257, 50000, (225, 320)), (2, 70000, (224, 300, 447, 448, 449))])
+def test_sample_tokens_top_k_around_the_lists_lengths(ops, dev, dtype, rows, V, tops):
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((rows, V)) * 2.5
+    x[0] = np.round(x[0] * 4) / 4                # few values, many ties at the cut
+    x[1, :400] += 9.0                            # the largest side by side
+    logits = torch.from_numpy(x).to(dev, dtype)
+    for k in tops:
+        check_sample(ops, dev, logits, rng.random(rows) * (1 - 2.0 ** -24), 1.0, k, 0.95, 0.001)
+        if rows < 9:
+            check_sample(ops, dev, logits, rng.random(rows) * (1 - 2.0 ** -24), 1.5, k, 1.0, 0.0)
+
+
 @pytest.mark.parametrize("V", [3000, 20000])
 def test_sample_tokens_of_peaked_rows(ops, dev, V):
     """Rows where a few logits hold the mass, also at one end of the row, with top-p alone and with everything."""
@@ -603,6 +619,7 @@ def test_sample_tokens_of_peaked_rows(ops, dev, V):
     x[3:6, V - 3:] += 12.0
     x[6, 77] = 60.0
     x[7] = np.floor(x[7])                       # few values, many ties
+    x[8], x[9] = np.sort(x[8]), -np.sort(x[9])  # in order
     for dtype in (torch.float32, torch.bfloat16):
         for s in SETTINGS:
             check_sample(ops, dev, torch.from_numpy(x).to(dev, dtype), rng.random(rows) * 0.999, *s, some=0.8)

@@ -220,7 +220,6 @@ __global__ __launch_bounds__(256) void sample_group_kernel(int64_t rows, int V, 
 
 // ---------------------------------------------------------------- longer rows: a workgroup per row
 constexpr int BINS = 512;                          // of log2 w, down to 2^-16
-constexpr int PAIRS = 256;                         // candidates that are compared each with each
 
 struct Candidate {
   u64 k;             // key << 32 | ~index: falling logits, equal ones by index
@@ -228,7 +227,10 @@ struct Candidate {
 };
 template <int NT>
 struct RowState {
-  static constexpr int NW = NT / 64, CAP = 1024;
+  // CAP: candidates of a list.  PAIRS: those that are compared each with each, more are sorted first (1 x 32000 with top-k 200: 18 us,
+  // up to 512 pairs 22; 1 x 131072 float32 with 256, 1024 threads: 40 up to 256 pairs, 31 up to 512).  FEW: top-k that such a
+  // list is for; what a list for more takes, the histogram takes too (512 x 65536, 224: 93 us against 133; 1 x 4000: 17 against 16)
+  static constexpr int NW = NT / 64, CAP = 1024, PAIRS = NT < 1024 ? 256 : 512, FEW = NT * 7 / 16;
   u64 list[CAP];
   union {
     u64 mass[NW][BINS];
@@ -276,50 +278,49 @@ __device__ __forceinline__ I block_scan(I v, I* s, I* sum) {
   return before + inc - v;
 }
 
-// sorts list[0 .. P), P a power of two: falling, or rising.  Up to WAVE_SORT a single wave does it, without barriers (256: 36
-// steps of about 0.06 us, where a barrier of 16 waves alone takes four times that)
-constexpr int WAVE_SORT = 512;
+// Sorts list[0 .. n), entries that all differ: falling, or rising.  Up to a thread's worth (and 512) every entry's place is
+// counted, all pairs compared; more (up to the next power of two, which the list has to hold) are sorted by exchanges, a barrier
+// for each step.  1 x 4000 with top-k 300: 16 us (exchanges alone 22, up to 128 of them by one wave 20); 4096 x 8000: 168 (191, 185).
 template <int NT>
-__device__ void sort_list(u64* list, int P, bool falling) {
-  const auto step = [&](int size, int stride, int from, int by) {
-    for (int i = from; i < P / 2; i += by) {
-      const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-      const u64 a = list[lo], b = list[hi];
-      if ((a < b) == (((lo & size) == 0) == falling) && a != b) { list[lo] = b; list[hi] = a; }
-    }
-  };
+__device__ void sort_list(u64* list, int n, bool falling) {
+  constexpr int RANKED = NT < 512 ? NT : 512;
+  const u64 flip = falling ? 0 : ~0ull;
+  const int tid = threadIdx.x;
   __syncthreads();
-  if (P <= WAVE_SORT) {
-    if (threadIdx.x < 64)
-      for (int size = 2; size <= P; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-          step(size, stride, threadIdx.x, 64);
-          lds_in_order();
-        }
+  if (n <= RANKED) {
+    const u64 mine = tid < n ? list[tid] ^ flip : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += (list[j] ^ flip) > mine;
+    __syncthreads();
+    if (tid < n) list[rank] = mine ^ flip;
     __syncthreads();
     return;
   }
+  int P = RANKED;
+  while (P < n) P <<= 1;
+  for (int i = n + tid; i < P; i += NT) list[i] = flip;
+  __syncthreads();
   for (int size = 2; size <= P; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      step(size, stride, threadIdx.x, NT);
+      for (int i = tid; i < P / 2; i += NT) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const u64 a = list[lo], b = list[hi];
+        if ((a < b) == (((lo & size) == 0) == falling) && a != b) { list[lo] = b; list[hi] = a; }
+      }
       __syncthreads();
     }
 }
-__device__ __forceinline__ int pow2_at_least(int n) {
-  int P = 64;
-  while (P < n) P <<= 1;
-  return P;
-}
 
-// A row with top-k of up to 512 takes two looks: the largest of every thread and piece, then the pieces that can hold a candidate;
+// A row with a small top-k takes two looks: the largest of every thread and piece, then the pieces that can hold a candidate;
 // top-p alone adds the exact sum of the row; all else the masses of the row by bins.  256 x 131072 bf16 with settings per row
-// (top-k about 64): 31 us (its argmax alone: 19), 1 x 32000: 11 us, of which 2 are the load and the rest steps that wait for
+// (top-k about 64): 27 us (its argmax alone: 15), 1 x 32000: 11 us, of which 2 are the load and the rest steps that wait for
 // each other.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V, const T* __restrict__ logits, int64_t ld, Settings st, int F,
                                                         const float* __restrict__ u, int64_t* __restrict__ out) {
   typedef RowState<NT> State;
-  constexpr int VEC = RowPieces<T>::VEC, NW = State::NW, CAP = State::CAP;
+  constexpr int VEC = RowPieces<T>::VEC, NW = State::NW, CAP = State::CAP, PAIRS = State::PAIRS, FEW = State::FEW;
   __shared__ State S;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
@@ -343,9 +344,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   }
 #define EACH(...) _Pragma("unroll") for (int e = 0; e < VEC; ++e) { __VA_ARGS__ }
 
-  // the thread's largest logit, the row's, and the smallest of the threads'
-  // top-p alone: the sum of the weights too, roughly (each thread relative to its own largest)
-  const bool guess = rs.T > 0.0 && !(rs.k > 0 && rs.k < V) && rs.p < 1.0 && V > CAP;
+  // The first look: the thread's largest logit, the row's, and the smallest of the threads'; every thread sees every NT-th piece,
+  // so that logits in falling order are spread too.  With top-p alone the sum of the weights as well, roughly (each thread's
+  // relative to its own largest).
+  const bool guess = rs.T > 0.0 && !(rs.k > 0 && rs.k < V) && rs.p < 1.0;
   const float rough = (float)rs.c;
   float tm = -INFINITY, tz = 0.f;
   const auto look = [&](const float (&v)[VEC]) {
@@ -363,21 +365,22 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   float most[H];
 #pragma unroll
   for (int h = 0; h < H; ++h) {
-    const int64_t i = lo + lane + 64 * h;
+    const int64_t i = tid + NT * h;
     most[h] = -INFINITY;
-    if (i < hi) {
+    if (i < row.np) {
       float v[VEC];
       row.load(i, v);
       look(v);
       EACH(most[h] = fmaxf(most[h], v[e]);)
     }
   }
-  for (int64_t i = lo + lane + 64 * H; i < hi; i += 64) {
+  for (int64_t i = tid + NT * H; i < row.np; i += NT) {
     float v[VEC];
     row.load(i, v);
     look(v);
   }
-  // The wave's pieces with an element that reaches f: S.piece[wave] has them, up to 64; returns how many there are.
+  // The pieces that the wave has seen with an element that reaches f: S.piece[wave] has them in order, up to 64; returns how many
+  // there are.
   const auto pieces_from = [&](float f) {
     int n = 0;
     const auto take = [&](bool in, int64_t i) {
@@ -388,16 +391,16 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     };
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      if (lo + 64 * h >= hi) break;
-      take(most[h] >= f, lo + lane + 64 * h);
+      if (NT * h >= row.np) break;
+      take(most[h] >= f, tid + NT * h);
     }
-    for (int64_t i0 = lo + 64 * H; i0 < hi; i0 += 64) {
+    for (int64_t i0 = NT * H; i0 < row.np; i0 += NT) {
       float v[VEC], b = -INFINITY;
-      if (i0 + lane < hi) {
-        row.load(i0 + lane, v);
+      if (i0 + tid < row.np) {
+        row.load(i0 + tid, v);
         EACH(b = fmaxf(b, v[e]);)
       }
-      take(b >= f, i0 + lane);
+      take(b >= f, i0 + tid);
     }
     lds_in_order();
     return n;
@@ -447,8 +450,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   // ---- few candidates: all that top-k can keep fits the list; or, with top-p alone, a guess: that the largest GUESS logits
   // hold top_p of the mass, as they do where a model is sure of its answers
   constexpr int GUESS = 160;
-  if ((by_k && rs.k <= CAP / 2 && rs.k <= NT) || ((by_k || by_p) && V <= CAP) || guess) {
-    const int64_t kk = by_k ? rs.k : guess ? GUESS : V;
+  if ((by_k && rs.k <= FEW) || guess) {
+    const int64_t kk = by_k ? rs.k : GUESS;
     // where kk threads' largest reach `floor`, at least kk logits do; not many more than kk are wanted
     // (the numbers of three values at a time, one barrier a step)
     float floor = -LARGEST;
@@ -463,7 +466,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       ++step;
       return all;
     };
-    if (V > CAP && (int64_t)(reach(least, least, least) & 0xffff) >= kk) {
+    if ((int64_t)(reach(least, least, least) & 0xffff) >= kk) {
       uint32_t a = key_of(least), b = key_of(m);
       while (a < b && step < 16) {
         const uint32_t k2 = between(a, b, step), k1 = between(a, k2, step), k3 = between(k2, b, step);
@@ -559,9 +562,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
     }
     if (n <= CAP) {
       // sorted: by logit for the cut, the kept ones by index for the answer
-      const int P = pow2_at_least(n);
-      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
-      sort_list<NT>(S.list, P, true);
+      sort_list<NT>(S.list, n, true);
       u64 whole = 0;
       if (by_p) {
         u64 w = 0;
@@ -583,13 +584,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
         above += sum;
       }
       // index << 32 | key, rising
-      const int Q = pow2_at_least((int)nkept);
       __syncthreads();
-      for (int i = tid; i < Q; i += NT) {
+      for (int i = tid; i < (int)nkept; i += NT) {
         const u64 a = S.list[i];
-        S.list[i] = i < (int)nkept ? (u64)(uint32_t)~(uint32_t)a << 32 | a >> 32 : ~0ull;
+        S.list[i] = (u64)(uint32_t)~(uint32_t)a << 32 | a >> 32;
       }
-      sort_list<NT>(S.list, Q, false);
+      sort_list<NT>(S.list, (int)nkept, false);
       const u64 target = target_of(uu, kept);
       u64 run = 0;
       for (int base = 0; base < (int)nkept; base += NT) {
@@ -665,9 +665,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
       }))
       __syncthreads();
       if (S.n > CAP) return false;
-      const int n = (int)S.n, P = pow2_at_least(n);
-      for (int i = n + tid; i < P; i += NT) S.list[i] = 0;
-      sort_list<NT>(S.list, P, true);
+      sort_list<NT>(S.list, (int)S.n, true);
       return true;
     };
     // the cut at the list's entry at which the number (or the mass, S.above of it above the list) reaches `want`
@@ -887,14 +885,22 @@ int launch_sample(int64_t rows, int64_t V, const void* logits, int64_t ld, const
   else if (V <= 2048) GROUP_(64, 32);
 #undef GROUP_
   else {
-    // One workgroup per row.  Up to a row for every CU the largest that the row feeds is the fastest (64 x 131072 bf16: 45 / 26 / 21
-    // us with 256 / 512 / 1024 threads; 1 x 32000: 16 / 14 / 15); with more rows small workgroups wait for each other's
-    // barriers less (4096 x 8000 bf16: 70 / 146 / 209 us; 1024 x 32000: 37 / 50 / 66; 512 x 65536: 35 / 33 / 43).
+    // One workgroup per row.  Up to a row for every CU the largest that the row feeds is the fastest (top-k 50, 64 x 131072 bf16:
+    // 44 / 26 / 20 us with 256 / 512 / 1024 threads; 1 x 32000: 13 / 11 / 13); with more rows small workgroups wait for each
+    // other's barriers less (4096 x 8000 bf16: 49 / 81 / 171 us; 1024 x 32000: 23 / 30 / 54; 512 x 65536: 30 / 22 / 35).
     const int64_t bytes = V * (int64_t)sizeof(T);
     const bool many = rows > 256;
+    int nt = many && bytes <= 98304 ? 256 : bytes <= (many ? 1 << 20 : 131072) ? 512 : 1024;
+    // The next larger one where its list of candidates has room for a top-k that this one's has not, up to 160 and (rows that feed
+    // it) 320 (4096 x 8000 float32, top-k 160: 150 us against 189, 200: 230 against 163; 1024 x 32000 bf16, 160: 49 against
+    // 115; 512 x 65536, 256: 69 against 133; 2000 x 65536 float32, 320: 367 against 480; 1 x 32000, 256: 25 against 41).
+    // Settings per row are not known here.
+    const int64_t k = st.kr || st.k >= V ? 0 : st.k;
+    if (nt == 256 && k > RowState<256>::FEW && k <= 160) nt = 512;
+    if (nt == 512 && k > RowState<512>::FEW && k <= 320 && bytes > (many ? 98304 : 49152)) nt = 1024;
 #define ROW_(NT) hipLaunchKernelGGL((sample_row_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, s, rows, V, x, ld, st, F, u, out)
-    if (many && bytes <= 98304) ROW_(256);
-    else if (bytes <= (many ? 1 << 20 : 131072)) ROW_(512);
+    if (nt == 256) ROW_(256);
+    else if (nt == 512) ROW_(512);
     else ROW_(1024);
 #undef ROW_
   }
