@@ -391,7 +391,8 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
 }
 
 // Runs that reach over the edges of chunks: a workgroup for each chunk in which one begins (the others leave at once) and
-// each 64 * VEC columns; its waves add every fourth part, and the four sums are added in order.  5 us where most leave.
+// each 64 * VEC columns; its waves add every fourth part, and the four sums are added in order.  4.6 us, loads that wait for
+// each other (5.3 with the parts asked for only when it is known which).
 template <int VEC>
 __global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, int64_t vocab, int P, int64_t nchunks, int ctiles, float scale,
                                                               int accumulate, const u64* __restrict__ keys, const float* __restrict__ part,
@@ -401,21 +402,33 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(int64_t n, int D, 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = ((int)(blockIdx.x - chunk * ctiles) * 64 + lane) * VEC;
   const int64_t a = chunk * P, b = a + P;                       // (not the last chunk: nothing goes on from there)
-  const uint32_t t = (uint32_t)(keys[b] >> 32);
-  if (t >= (uint64_t)vocab || (uint32_t)(keys[b - 1] >> 32) != t || (a > 0 && (uint32_t)(keys[a - 1] >> 32) == t)) return;
+  // the tokens that decide and the wave's first parts are asked for together (parts that turn out not to be are not used)
+  const auto begins = [&](int64_t k) { return (uint32_t)(keys[(k < nchunks ? k : chunk) * P] >> 32); };
+  const uint32_t t = (uint32_t)(keys[b] >> 32), at_end = (uint32_t)(keys[b - 1] >> 32), at_start = a > 0 ? (uint32_t)(keys[a - 1] >> 32) : UINT_MAX;
+  uint32_t next = begins(chunk + 1 + lane);
+  float own[VEC] = {}, one[VEC] = {};
+  if (c < D) {
+    if (wave == 0) load_pack<float, VEC>(part + (2 * chunk + 1) * D + c, own);
+    if (chunk + 1 + wave < nchunks) load_pack<float, VEC>(part + (2 * (chunk + 1 + wave)) * D + c, one);
+  }
+  if (t >= (uint64_t)vocab || at_end != t || at_start == t) return;
   int64_t last = chunk;                                         // the last chunk that begins inside the run
-  for (bool more = true; more;) {
-    const int64_t k = last + 1 + lane;
-    const u64 in = __ballot(k < nchunks && (uint32_t)(keys[k < nchunks ? k * P : 0] >> 32) == t);
-    const int ahead = in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
-    last += ahead;
-    more = ahead == 64;
+  for (;;) {
+    const u64 in = __ballot(last + 1 + lane < nchunks && next == t);
+    last += in == ~0ull ? 64 : __ffsll((long long)~in) - 1;
+    if (in != ~0ull) break;
+    next = begins(last + 1 + lane);
   }
   float acc[VEC] = {};
   if (c < D) {
-    if (wave == 0) load_pack<float, VEC>(part + (2 * chunk + 1) * D + c, acc);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = wave == 0 ? own[i] : 0.f;
+    if (chunk + 1 + wave <= last) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += one[i];
+    }
 #pragma unroll 8
-    for (int64_t k = chunk + 1 + wave; k <= last; k += 4) {
+    for (int64_t k = chunk + 5 + wave; k <= last; k += 4) {
       float v[VEC];
       load_pack<float, VEC>(part + (2 * k) * D + c, v);
 #pragma unroll
