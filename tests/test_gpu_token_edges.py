@@ -1,0 +1,91 @@
+"""Token family where it can go wrong: sums of whole numbers, which leave a gradient no tolerance, over every form of its
+sort and cut; workspaces of exactly the stated size whatever they hold; teacher's entries on masked logits; rows cut out of
+wider tensors; draws of infinite logits, and next to a border.
+
+Restatement: oracle/tokens.py.  e = 2^-24 is half a float32 step."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import tokens as otok
+
+pytestmark = pytest.mark.gpu
+
+E24 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need an MI355X"
+    return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def ops(lib):
+    from timeautodiff_amd import ops as _ops
+    return _ops
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def tokens_of(kind, n, V, rng):
+    if kind == "same":
+        return np.full(n, V // 2)
+    if kind == "padding":
+        return np.full(n, V + 3)
+    if kind == "spread":
+        return rng.integers(0, V, n)
+    tok = np.minimum(((V + 1.0) ** rng.random(n)).astype(np.int64) - 1, V - 1)
+    if kind == "ragged":
+        tok[rng.random(n) < 0.3] = rng.choice([-1, V, 1 << 40])
+        tok[n - n // 5:] = -1
+    return tok
+
+
+# ------------------------------------------------------------------ distillation
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [6, 48, 700, 9000])
+def test_distill_loss_of_entries_on_masked_logits(ops, dev, dtype, V):
+    """A logit masked with the type's lowest value is finite: p = 0 there, and the loss of an entry on it is w tau q (max - logit) to
+    within the others' share, finite wherever float32 holds it.  q is off by e (16 A + K + 64) relative, A the range of value /
+    tau; four roundings more."""
+    rng = np.random.default_rng(V)
+    rows, K = 12, 5
+    for tau in (1.0, 0.25, 3.0):
+        x = rng.standard_normal((rows, V)) * 2.5
+        logits = torch.from_numpy(x).to(dev, dtype)
+        low = torch.finfo(dtype).min
+        logits[:, 1], logits[:, V - 1] = low, low
+        index = np.tile(np.array([0, 1, 2, V - 1, 3]), (rows, 1))
+        value = rng.standard_normal((rows, K)).astype(np.float32)
+        index[0] = [1, 1, V - 1, 1, V - 1]                       # every entry on a masked logit
+        logits[1, 2] = -low                                      # max - logit itself is more than float32 holds
+        weight = rng.uniform(0.02, 0.3, rows).astype(np.float32)
+        weight[2] = 8.0
+        loss, d = torch.empty(rows, device=dev), torch.empty(rows, V, dtype=dtype, device=dev)
+        ops.distill_loss(logits, torch.from_numpy(index).to(dev), torch.from_numpy(value).to(dev), loss, temperature=tau,
+                         row_weight=torch.from_numpy(weight).to(dev), dlogits=d)
+        want, grad = otok.distill(f64(logits), index, value, tau, weight, 1.0)
+        got = f64(loss)
+        most = float(np.finfo(np.float32).max)
+        A = float(np.ptp(value, axis=1).max()) / tau
+        rel = E24 * (16 * A + K + 64 + 4)
+        fits, over = want < most * (1 - rel), want > most * (1 + rel)
+        assert fits.sum() >= 8 and np.all(fits | over)
+        assert np.all(np.isinf(got[over]) & (got[over] > 0))
+        assert np.all(np.abs(got[fits] - want[fits]) <= rel * want[fits]), (got, want)
+        # p as in the loss of any other row: arguments of up to A' = range of the live logits / tau
+        live = np.ptp(x, axis=1).max() / tau + np.log(V)
+        err = E24 * (16 * max(A, live) + V / 32 + K + 64)
+        for r in range(rows):
+            if r == 1:
+                continue                                         # (its largest logit holds all of p)
+            q = np.exp(value[r].astype(np.float64) / tau)
+            q /= q.sum()
+            qq = np.zeros(V)
+            np.add.at(qq, index[r], q)
+            g = weight[r] * tau
+            tol = g * 2 * err * (np.abs(grad[r]) / g + 2 * qq) + ((2.0 ** -8 if dtype == torch.bfloat16 else E24) + 3 * E24) * np.abs(grad[r]) + 1e-37
+            assert np.all(np.abs(f64(d[r]) - grad[r]) <= tol), r

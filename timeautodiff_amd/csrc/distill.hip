@@ -5,7 +5,11 @@
 //   loss[r] = w_r tau^2 sum_k q_k (ln q_k - ln p[index_k]),   dlogits[r, j] = grad_scale w_r tau (p_j - sum of the q_k with index_k = j)
 //
 // Statistics and sums in fp32, exponentials as 2^((x - max) log2(e) / tau) on the hardware's exp2 (the difference before the
-// product: a row of the type's lowest values stays a row of zeros).
+// product: a row of the type's lowest values stays a row of zeros).  The loss is added up in the logits' own units, at half scale:
+//
+//   loss[r] = 2 w tau sum_k q_k ((value_k / 2 - max / 2) - (logit_k / 2 - max / 2) - tau / 2 (ln sum_teacher - ln sum_student))
+//
+// so that no part of it leaves fp32's range where the loss itself does not (an entry on a logit masked with the lowest value).
 #include <limits.h>
 #include <math.h>
 
@@ -29,6 +33,8 @@ struct Args {
 };
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+// (x - largest) / 2, rounded once; finite for all finite x
+__device__ __forceinline__ float half_from(float x, float largest) { return __builtin_fmaf(0.5f, x, -0.5f * largest); }
 
 // ---------------------------------------------------------------- short rows: G lanes of a wave per row
 // The row stays in registers (E logits a lane), statistics go across the G lanes by DPP, and the teacher's q reach their
@@ -77,15 +83,15 @@ __global__ __launch_bounds__(256) void distill_short_kernel(Args A, const T* log
   z = across<G, Add>(z);
   tz = across<G, Add>(tz);
   const bool counts = w != 0.f && z != 0.f && tz != 0.f;
-  const float itz = 1.f / tz, l2 = __log2f(tz) - __log2f(z);
-  const auto term = [&](float q, float t, float s) { return q > 0.f ? q * ((t - tm) * A.c - (s - m) * A.c - l2) : 0.f; };
+  const float itz = 1.f / tz, lz = 0.5f * A.tau * LN2 * (__log2f(tz) - __log2f(z));
+  const auto term = [&](float q, float t, float s) { return q > 0.f ? q * (half_from(t, tm) - half_from(s, m) - lz) : 0.f; };
   float l = i0 >= 0 ? term(q0 * itz, v0, x0) : 0.f;
   for (int k = lane + G; k < A.K; k += G) {
     const int i = entry(k);
     if (i >= 0) l += term(ex2((val[k] - tm) * A.c) * itz, val[k], (float)x[i]);
   }
   l = across<G, Add>(l);
-  if (lane == 0) A.loss[r] = counts ? w * A.tau * A.tau * (l * LN2) : 0.f;
+  if (lane == 0) A.loss[r] = counts ? 2.f * (w * A.tau * l) : 0.f;
   if (!dlogits) return;
   uint32_t* mine = tgt[slot];
   if (i0 >= 0) mine[i0] = lane;
@@ -230,21 +236,20 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
       for (int64_t j = tid; j < V; j += NT) d[j] = (T)0.f;
     return;
   }
-  const float itz = 1.f / tz, iz = 1.f / z, l2 = __log2f(tz) - __log2f(z), g = A.grad_scale * w * A.tau;
+  const float itz = 1.f / tz, iz = 1.f / z, lz = 0.5f * A.tau * LN2 * (__log2f(tz) - __log2f(z)), g = A.grad_scale * w * A.tau;
   float l = 0.f, unused = 0.f;
 #pragma unroll
   for (int n = 0; n < KE; ++n) {
-    const float b = (xv[n] - m) * A.c;
-    p[n] = ex2(b) * iz;
+    p[n] = ex2((xv[n] - m) * A.c) * iz;
     qn[n] *= itz;
-    if (qn[n] > 0.f) l += qn[n] * ((val[n] - tm) * A.c - b - l2);
+    if (qn[n] > 0.f) l += qn[n] * (half_from(val[n], tm) - half_from(xv[n], m) - lz);
     if (tid + n * NT < K) {
       q[tid + n * NT] = qn[n];
       at[tid + n * NT] = mine[n];
     }
   }
   block_two<NW, false>(l, unused, red);
-  if (tid == 0) A.loss[r] = w * A.tau * A.tau * (l * LN2);
+  if (tid == 0) A.loss[r] = 2.f * (w * A.tau * l);
   if (!d) return;
   const float gz = g * iz;
   const auto put = [&](int64_t i, const pack& p) {
