@@ -44,6 +44,22 @@ def tokens_of(kind, n, V, rng):
     return tok
 
 
+@pytest.mark.parametrize("n", [300, 9000])
+def test_accumulating_gradient_of_a_very_large_table(ops, dev, n):
+    """Rows of a table of more than 2^29 that no token names are not touched, so their number costs nothing."""
+    V = (1 << 29) + 7
+    rng = np.random.default_rng(n)
+    tok = rng.integers(0, V, n)
+    tok[::3] = V - 1 - rng.integers(0, 40, tok[::3].size)
+    terms = rng.integers(1, 9, n)
+    table = torch.zeros(V, 1, device=dev)
+    ops.token_embed_bwd(torch.from_numpy(tok).to(dev), torch.from_numpy(terms).to(dev).float().view(n, 1), table)
+    at, inverse = np.unique(tok, return_inverse=True)
+    want = np.bincount(inverse, weights=terms)
+    assert np.array_equal(f64(table[torch.from_numpy(at).to(dev), 0]), want)
+    assert int(torch.count_nonzero(table)) == at.size
+
+
 # ------------------------------------------------------------------ distillation
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [6, 48, 700, 9000])

@@ -502,6 +502,9 @@ __global__ __launch_bounds__(DIRECT_WAVES * 64) void embed_grad_direct_kernel(in
 }
 
 // ---------------------------------------------------------------- host side
+// workgroups that write the rows which no token names (overwriting mode only)
+inline int64_t zero_groups(int64_t vocab, int accumulate) { return accumulate ? 0 : cdiv64(vocab, ZROWS * GW); }
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr int64_t COUNT_BYTES = MAX_TILES * MAX_BINS * 4;
@@ -561,7 +564,7 @@ void launch_direct(int64_t n, int D, int64_t vocab, const int64_t* tok, int64_t 
 template <typename T, int VEC, int M>
 void launch_sum(const GradPlan& g, int64_t n, int D, int64_t vocab, float scale, int accumulate, const u64* keys, const void* dout, int64_t ldd,
                 float* dtable, int64_t ldg, float* part, hipStream_t s) {
-  const int64_t grid = g.nchunks * g.ctiles + (accumulate ? 0 : cdiv64(vocab, ZROWS * GW));
+  const int64_t grid = g.nchunks * g.ctiles + zero_groups(vocab, accumulate);
   hipLaunchKernelGGL((embed_grad_sum_kernel<T, VEC, M>), dim3((unsigned)grid), dim3(GW * 64), 0, s, n, D, vocab, g.S, g.nchunks, g.ctiles, scale,
                      accumulate, keys, (const T*)dout, ldd, dtable, ldg, part);
 }
@@ -612,7 +615,7 @@ extern "C" int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_
   const int64_t kb = key_bytes(n);
   TAD_CHECK(workspace && aligned16(workspace) && workspace_bytes >= 2 * kb + COUNT_BYTES + 2 * g.nchunks * D * 4,
             "tad_token_embed_bwd: workspace of %lld bytes, 16-byte aligned, needed", (long long)tad_token_embed_bwd_workspace_bytes(n, D));
-  TAD_CHECK(g.nchunks * g.ctiles + cdiv64(vocab, ZROWS * GW) < (1 << 23) && g.nchunks * cdiv64(D, wide ? 256 : 64) < (1 << 24),
+  TAD_CHECK(g.nchunks * g.ctiles + zero_groups(vocab, accumulate) < (1 << 23) && g.nchunks * cdiv64(D, wide ? 256 : 64) < (1 << 24),
             "tad_token_embed_bwd: too many tokens or rows");                        // (a grid holds fewer than 2^32 threads)
   // the direct form, where its workgroups are few (2048: two rounds of the chip), read the tokens few times (2^22: 32 MB from L2)
   // and a row of the table does not get so many tokens that the one workgroup's time is theirs (2400 tokens of 128 columns
