@@ -105,3 +105,24 @@ def test_distill_loss_of_entries_on_masked_logits(ops, dev, dtype, V):
             g = weight[r] * tau
             tol = g * 2 * err * (np.abs(grad[r]) / g + 2 * qq) + ((2.0 ** -8 if dtype == torch.bfloat16 else E24) + 3 * E24) * np.abs(grad[r]) + 1e-37
             assert np.all(np.abs(f64(d[r]) - grad[r]) <= tol), r
+
+
+# ------------------------------------------------------------------ draw
+@pytest.mark.parametrize("V", [12, 100, 3000, 40000])
+def test_infinite_logits_count_as_the_largest_number(ops, dev, V):
+    """+inf is the largest float32 number: the two tie, and the lowest index is taken."""
+    logits = torch.randn(3, V, device=dev)
+    most = torch.finfo(torch.float32).max
+    logits[0, V - 2], logits[0, 5] = float("inf"), most
+    logits[1, 4], logits[1, V - 1] = float("inf"), most
+    logits[2, 7], logits[2, V - 3] = most, most
+    out = torch.empty(3, dtype=torch.int64, device=dev)
+    ops.sample_tokens(logits, torch.rand(3, device=dev), out, temperature=0.0)
+    assert out.tolist() == [5, 4, 7]
+    for opt in (dict(), dict(top_k=3), dict(top_p=0.9), dict(min_p=0.5)):
+        ops.sample_tokens(logits, torch.zeros(3, device=dev), out, **opt)
+        assert out.tolist() == [5, 4, 7], opt
+        ops.sample_tokens(logits, torch.full((3,), 0.999, device=dev), out, **opt)
+        assert out.tolist() == [V - 2, V - 1, V - 3], opt
+    ops.sample_tokens(logits, torch.full((3,), 0.999, device=dev), out, top_k=1)
+    assert out.tolist() == [5, 4, 7]

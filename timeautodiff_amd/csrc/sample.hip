@@ -423,11 +423,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(int64_t rows, int64_t V,
   }
   if (!(rs.T > 0.0)) {
     u64 at = ~0ull;                         // the lowest index of the largest (pieces come in order: the first that has it)
-    if (pieces_from(m) > 0) {
+    const float top = fminf(m, LARGEST);
+    if (pieces_from(top) > 0) {
       const int64_t i = S.piece[wave][0];
       float v[VEC];
       row.load(i, v);
-      EACH(if (v[VEC - 1 - e] == m) at = (u64)(row.first(i) + VEC - 1 - e);)
+      EACH(if (v[VEC - 1 - e] >= top) at = (u64)(row.first(i) + VEC - 1 - e);)
     }
     at = across<64, Min>(at);
     if (lane == 0) S.wsum[wave] = at;
