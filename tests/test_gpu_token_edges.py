@@ -107,6 +107,35 @@ def test_distill_loss_of_entries_on_masked_logits(ops, dev, dtype, V):
             assert np.all(np.abs(f64(d[r]) - grad[r]) <= tol), r
 
 
+# ------------------------------------------------------------------ rows out of wider tensors
+@pytest.mark.parametrize("B,T,V", [(4, 5, 300), (3, 1, 40), (1, 6, 17)])
+def test_last_step_of_a_sequence(ops, dev, B, T, V):
+    """x[:, -1:, :] has the rows of x[:, -1, :]: a dimension of one element has no stride of its own."""
+    rng = np.random.default_rng(B * T)
+    x = torch.from_numpy(rng.standard_normal((B, T, V)).astype(np.float32)).to(dev)
+    a, b = x[:, -1:, :], x[:, -1, :]
+    u = torch.rand(B, device=dev)
+    got, want = torch.empty(B, 1, dtype=torch.int64, device=dev), torch.empty(B, dtype=torch.int64, device=dev)
+    ops.sample_tokens(a, u, got, top_p=0.9)
+    ops.sample_tokens(b, u, want, top_p=0.9)
+    assert torch.equal(got.view(-1), want)
+    index, value = torch.randint(0, V, (B, 1, 3), device=dev), torch.randn(B, 1, 3, device=dev)
+    da, db = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    la, lb = torch.empty(B, 1, device=dev), torch.empty(B, device=dev)
+    ops.distill_loss(a, index, value, la, dlogits=da[:, -1:, :])
+    ops.distill_loss(b, index[:, 0], value[:, 0], lb, dlogits=db[:, -1, :])
+    assert torch.equal(la.view(-1), lb) and torch.equal(da, db)
+    table, tok = torch.randn(9, V, device=dev), torch.randint(0, 9, (B, 1), device=dev)
+    ops.token_embed_fwd(tok, table, da[:, -1:, :])
+    assert torch.equal(da[:, -1], table[tok[:, 0]]) and bool((da[:, :-1] == 7.0).all())
+    ga, gb = torch.empty_like(table), torch.empty_like(table)
+    ops.token_embed_bwd(tok, a, ga, accumulate=False)
+    ops.token_embed_bwd(tok[:, 0], b, gb, accumulate=False)
+    assert torch.equal(ga, gb)
+    with pytest.raises(AssertionError):                          # two strides: no rows
+        ops.sample_tokens(torch.zeros(4, 6, V, device=dev)[:, :3], torch.rand(12, device=dev), torch.empty(12, dtype=torch.int64, device=dev))
+
+
 # ------------------------------------------------------------------ draw
 @pytest.mark.parametrize("V", [12, 100, 3000, 40000])
 def test_infinite_logits_count_as_the_largest_number(ops, dev, V):

@@ -85,11 +85,14 @@ def as2d(t, dtype=torch.float32):
     if t.dim() == 1:
         return t.data_ptr(), 1, cols, cols
     ld = t.stride(-2) if t.shape[-2] > 1 else max(cols, t.stride(-2))
-    expect = ld * t.shape[-2]
+    # the rows' stride is that of the innermost leading dimension with more than one element (one of one element has none)
+    expect = ld * t.shape[-2] if t.shape[-2] > 1 else None
     for d in range(t.dim() - 3, -1, -1):
         if t.shape[d] > 1:
+            if expect is None:
+                ld = expect = t.stride(d)
             assert t.stride(d) == expect, ("leading dims do not collapse", t.shape, t.stride())
-        expect *= t.shape[d]
+            expect *= t.shape[d]
     return t.data_ptr(), t.numel() // cols, cols, ld
 
 
