@@ -576,6 +576,7 @@ extern "C" int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_
   TAD_CHECK(n >= 0 && D >= 1 && vocab >= 0, "tad_token_embed_fwd: bad sizes");
   TAD_CHECK((table_dtype == TAD_F32 || table_dtype == TAD_BF16) && (out_dtype == TAD_F32 || out_dtype == TAD_BF16), "tad_token_embed_fwd: bad element type");
   TAD_CHECK(ld_table >= D && ldo >= D && tok_stride >= 0, "tad_token_embed_fwd: bad leading dimension");
+  TAD_CHECK(n < (int64_t)1 << 40, "tad_token_embed_fwd: too many tokens");        // (the sizes of the launch are formed in 64 bits)
   if (n == 0) return TAD_OK;
   TAD_CHECK(tokens && out && (table || vocab == 0), "tad_token_embed_fwd: null pointer");
   hipStream_t s = (hipStream_t)stream;
