@@ -44,6 +44,56 @@ def tokens_of(kind, n, V, rng):
     return tok
 
 
+# ------------------------------------------------------------------ gradient of the lookup
+# one launch (n <= 4096 and few rows); all pairs compared (n <= 8192); digits: one of 9 bits with every bin in use (511 rows and
+# padding), two of 5 and of 9, three of 7; waves of 64 positions (270000); one, two, four columns a lane, two packs of four (bf16)
+GRADIENTS = [(4096, 100, 256, torch.float32), (4096, 3, 260, torch.bfloat16), (4097, 40, 128, torch.float32), (8192, 500, 128, torch.bfloat16),
+             (8193, 500, 128, torch.float32), (8193, 3, 520, torch.bfloat16), (20000, 511, 520, torch.bfloat16), (20000, 512, 260, torch.float32),
+             (20001, 131072, 128, torch.float32), (20000, 300000, 20, torch.bfloat16), (70001, 37, 256, torch.bfloat16), (70001, 4000, 132, torch.float32),
+             (140001, 1000, 3, torch.float32), (270000, 1000, 8, torch.float32)]
+
+
+@pytest.mark.parametrize("kind", ["zipf", "ragged", "same", "spread", "padding"])
+@pytest.mark.parametrize("n,V,D,dtype", GRADIENTS)
+def test_gradient_of_whole_numbers_is_exact(ops, dev, kind, n, V, D, dtype):
+    """Terms 1 .. 8 and a scale of 1/2: every sum is exact in any order (270000 * 8 < 2^24), so a row, a chunk or an edge left
+    out or taken twice shows whatever the length of a run."""
+    rng = np.random.default_rng(n + V + D)
+    tok = torch.from_numpy(tokens_of(kind, n, V, rng))
+    terms = torch.from_numpy(rng.integers(1, 9, (n, D)))
+    fine = (tok >= 0) & (tok < V)
+    want = torch.zeros(V, D, dtype=torch.int64).index_add_(0, tok[fine], terms[fine]).to(dev).double() * 0.5
+    for extra in (0, 3):
+        wide = torch.full((n, D + extra), float("nan"), dtype=dtype, device=dev)
+        dout = wide[:, :D]
+        dout.copy_(terms.to(dev))
+        dout[~fine.to(dev)] = float("nan")                      # what padding holds has no share
+        table = torch.full((V, D + extra), 3.0, device=dev)
+        for accumulate in (False, True):
+            table.fill_(3.0)
+            ops.token_embed_bwd(tok.to(dev), dout, table[:, :D], scale=0.5, accumulate=accumulate)
+            assert torch.equal(table[:, :D].double(), want + 3.0 if accumulate else want)
+            assert bool((table[:, D:] == 3.0).all())
+
+
+@pytest.mark.parametrize("n,V,D,dtype", GRADIENTS)
+def test_gradient_of_long_runs(ops, dev, n, V, D, dtype):
+    """A term goes through at most 256 additions of the one launch, or 64 of its wave, 8 of the workgroup and one for every fourth
+    chunk of 64 or more positions: 300 + n / 256 roundings, whatever the number of a row's terms; twice, the same bits."""
+    rng = np.random.default_rng(n)
+    x = torch.from_numpy(rng.standard_normal((n, D)).astype(np.float32)).to(dev, dtype)
+    for kind in ("same", "zipf"):
+        tok = torch.from_numpy(tokens_of(kind, n, V, rng)).to(dev)
+        a, b = torch.empty(V, D, device=dev), torch.empty(V, D, device=dev)
+        ops.token_embed_bwd(tok, x, a, scale=1.25, accumulate=False)
+        ops.token_embed_bwd(tok, x, b, scale=1.25, accumulate=False)
+        assert torch.equal(a, b)
+        d, t = x.cpu().double(), tok.cpu()
+        want = torch.zeros(V, D, dtype=torch.float64).index_add_(0, t, d) * 1.25
+        size = torch.zeros(V, D, dtype=torch.float64).index_add_(0, t, d.abs()) * 1.25
+        assert bool(((a.cpu().double() - want).abs() <= E24 * (300 + n / 256) * size).all())
+
+
 @pytest.mark.parametrize("n", [300, 9000])
 def test_accumulating_gradient_of_a_very_large_table(ops, dev, n):
     """Rows of a table of more than 2^29 that no token names are not touched, so their number costs nothing."""
