@@ -577,8 +577,8 @@ int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, 
  * names it); with it the rows that no token names are not touched.  Padding tokens have no share.  The sums are float32 in a
  * fixed order that the tokens alone decide: the same bits from every call.  n < 2^31, vocab < 2^31 - 1, and so
  * many that no launch has 2^32 threads (a fault of size is an error).
- * workspace: tad_token_embed_bwd_workspace_bytes(n, D) bytes, 16-byte aligned, not read before it is written; calls that
- * overlap on the device (and graphs that may) need workspaces of their own. */
+ * workspace: tad_token_embed_bwd_workspace_bytes(n, D) bytes, 16-byte aligned; what it holds before the call changes nothing; calls
+ * that overlap on the device (and graphs that may) need workspaces of their own. */
 int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D);
 int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, int64_t tok_stride, float scale, const void* dout,
                         int dout_dtype, int64_t ld_dout, float* dtable, int64_t ld_dtable, int accumulate, void* workspace,

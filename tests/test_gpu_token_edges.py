@@ -110,6 +110,27 @@ def test_accumulating_gradient_of_a_very_large_table(ops, dev, n):
     assert int(torch.count_nonzero(table)) == at.size
 
 
+@pytest.mark.parametrize("n,V,D,dtype", [(4096, 3, 9, torch.float32), (5000, 40, 9, torch.float32), (5000, 5000, 128, torch.bfloat16), (8192, 2, 520, torch.bfloat16),
+                                         (9001, 500, 520, torch.bfloat16), (9001, 300000, 4, torch.float32), (70001, 3, 128, torch.float32),
+                                         (70001, 70000, 9, torch.bfloat16)])
+def test_gradient_in_a_workspace_of_the_stated_size(ops, dev, n, V, D, dtype):
+    """Forms that sort and join: nothing is written beside the workspace, and what it holds before the call changes nothing."""
+    rng = np.random.default_rng(n + D)
+    nb = ops.token_embed_bwd_workspace_bytes(n, D)
+    buf = torch.empty(nb + 512, dtype=torch.uint8, device=dev)
+    for kind in ("zipf", "same"):
+        tok = torch.from_numpy(tokens_of(kind, n, V, rng)).to(dev)
+        for extra in (0, 4, 3):
+            dout = torch.from_numpy(rng.standard_normal((n, D + extra))).to(dev, dtype)[:, :D]
+            want, got = torch.empty(V, D, device=dev), torch.empty(V, D, device=dev)
+            ops.token_embed_bwd(tok, dout, want, accumulate=False)
+            for held in (0xAB, 0xFF, 0x00):                     # (0xFF: every float32 in it a NaN)
+                buf.fill_(held)
+                ops.token_embed_bwd(tok, dout, got, accumulate=False, workspace=buf[256:256 + nb])
+                assert torch.equal(want, got)
+                assert bool((buf[:256] == held).all()) and bool((buf[256 + nb:] == held).all())
+
+
 # ------------------------------------------------------------------ distillation
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [6, 48, 700, 9000])
