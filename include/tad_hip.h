@@ -568,15 +568,16 @@ int tad_flip_categories(int64_t rows, int64_t F, int n_cols, const int32_t* cols
  * Tokens and indices are int64. */
 
 /* out[i, :] = scale * table[tokens[i * tok_stride], :], i < n; table [vocab, D] and out [n, D] float32 or bf16 (table_dtype,
- * out_dtype), any row strides >= D (16-byte aligned bases and D, ld multiples of 8 (both bf16) or 4 move 16 bytes a lane).
+ * out_dtype), any row strides >= D (16-byte aligned bases with D, ld multiples of 4, where either is bf16 of 8, move 16 bytes
+ * a lane or more, others one element).
  * A token outside [0, vocab) is padding: its row of out is zeros.  The product is formed in float32 and rounded once. */
 int tad_token_embed_fwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, int64_t tok_stride, float scale, const void* table,
                         int table_dtype, int64_t ld_table, void* out, int out_dtype, int64_t ldo, tad_stream_t stream);
 /* Its gradient: dtable[v, :] = (accumulate: +=) scale * sum over the i with tokens[i * tok_stride] = v of dout[i, :]; dout
  * [n, D] float32 or bf16, dtable [vocab, D] float32.  Without accumulate every row of dtable is written (zeros where no token
- * names it); with it the rows that no token names are not touched.  Padding tokens have no share.  The sums are float32 in a
- * fixed order that the tokens alone decide: the same bits from every call.  n < 2^31, vocab < 2^31 - 1, and so
- * many that no launch has 2^32 threads (a fault of size is an error).
+ * names it); with it the rows that no token names are not touched.  Padding tokens have no share.  The sums are float32 in an
+ * order that the tokens, the sizes, dout's type and whether packs of 4 columns are aligned decide: the same bits from every such call.
+ * n < 2^31, vocab < 2^31 - 1, and so many that no launch has 2^32 threads (a fault of size is an error).
  * workspace: tad_token_embed_bwd_workspace_bytes(n, D) bytes, 16-byte aligned; what it holds before the call changes nothing; calls
  * that overlap on the device (and graphs that may) need workspaces of their own. */
 int64_t tad_token_embed_bwd_workspace_bytes(int64_t n, int D);
