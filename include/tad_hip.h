@@ -606,9 +606,10 @@ int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dty
  * Ties go to the lowest index.  T = 0 takes the largest logit.  -inf and NaN logits are never drawn; a row with no other
  * gives -1; +inf counts as the largest float32 number.  Each setting is one number, or, where its _rows pointer is given, a number
  * per row (T, top_p, min_p float32, top_k int32; there T not above 0 means 0, top_k below 1 means all, min_p above 1 means 1;
- * NaN: T 0, the others off).  u below 0 or NaN counts as 0, u of 1 or more gives the last kept token.  The masses are
- * whole multiples of 2^-F of the largest weight (F = 44; 61 - log2 V above 2^17 logits, 53 - log2 V from 512 to 2048): every
- * sum is exact. */
+ * NaN: T 0, the others off).  u below 0 or NaN counts as 0, u of 1 or more gives the last kept token that has a mass.  The
+ * masses are whole multiples of 2^-F of the largest weight (F = 44; 61 - log2 V above 2^17 logits, 53 - log2 V from 513 to 2048,
+ * log2 rounded up): every sum is exact, and the answer that of the real numbers unless u times the kept sum, or top_p times its
+ * own, lies closer to a border than V 2^-(F+1) times the largest weight.  A weight below 2^-(F+1) of the largest has no mass. */
 int tad_sample_tokens(int64_t rows, int64_t V, const void* logits, int dtype, int64_t ld, double temperature, const float* temperature_rows,
                       int64_t top_k, const int32_t* top_k_rows, double top_p, const float* top_p_rows, double min_p,
                       const float* min_p_rows, const float* u, int64_t* out, tad_stream_t stream);

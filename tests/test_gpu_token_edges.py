@@ -226,3 +226,43 @@ def test_infinite_logits_count_as_the_largest_number(ops, dev, V):
         assert out.tolist() == [V - 2, V - 1, V - 3], opt
     ops.sample_tokens(logits, torch.full((3,), 0.999, device=dev), out, top_k=1)
     assert out.tolist() == [5, 4, 7]
+
+
+@pytest.mark.parametrize("V,F", [(500, 44), (2048, 42), (32000, 44), (131072, 44), (300000, 42)])
+def test_draw_next_to_a_border(ops, dev, V, F):
+    """One logit leads and all others are equal, so that their weights are rounded alike and the roundings add up.  Each weight is
+    off by at most 2^-(F+1) of the largest, so a border by at most V times that (u times the sum is a whole number of 2^-F too: 4
+    more); sums in float64 to 2^-48 of them."""
+    N = 64
+    # (tails that hold a share of the row, next to which 2^-(F+1) is small)
+    for tail in (-6.0, -18.0):
+        w = np.exp(tail)
+        for lead in (0, V // 3, V - 1):
+            row = torch.full((V,), tail, device=dev)
+            row[lead] = 0.0
+            c = np.arange(1, V + 1) * w
+            c[lead:] += 1.0 - w
+            # numbers that fall among the tail before the leader and behind it, where there are any
+            before, behind = lead * w / c[-1], 1.0 - (V - 1 - lead) * w / c[-1]
+            g = np.random.default_rng(V + lead)
+            u = np.concatenate([g.uniform(0.0, max(before, 1e-9), N // 2), g.uniform(min(behind, 1 - 1e-7), 1.0, N // 2)]).astype(np.float32)
+            u = np.minimum(u, np.float32(1 - E24))
+            for dtype in (torch.bfloat16, torch.float32):
+                out = torch.empty(N, dtype=torch.int64, device=dev)
+                ops.sample_tokens(row.to(dtype).expand(N, V).contiguous(), torch.from_numpy(u).to(dev), out)
+                at = out.cpu().numpy()
+                off = (V + 4) * 2.0 ** -(F + 1) + c[-1] * 2.0 ** -48
+                target = u.astype(np.float64) * c[-1]
+                assert np.all(target <= c[at] + off) and np.all(target >= np.where(at > 0, c[at - 1], 0.0) - off)
+
+
+@pytest.mark.parametrize("V", [30, 700, 5000])
+def test_weights_below_half_a_unit_are_never_drawn(ops, dev, V):
+    """e^-40 is below 2^-45: such a logit is kept by a filter that counts, and has no mass."""
+    logits = torch.full((3, V), -40.0, device=dev)
+    logits[:, 3] = 0.0
+    u = torch.tensor([0.0, 0.5, 1.0], device=dev)
+    out = torch.empty(3, dtype=torch.int64, device=dev)
+    for opt in (dict(), dict(top_k=10), dict(top_p=0.99), dict(top_k=10, min_p=1e-30)):
+        ops.sample_tokens(logits, u, out, **opt)
+        assert out.tolist() == [3, 3, 3], opt

@@ -6,9 +6,12 @@
 //
 // The answer is an index that a sum decides, so the sums are exact: every w is rounded once to a whole multiple of 2^-F (F =
 // 44 for rows of up to 512 logits and of 2049 to 2^17, else a few less) and added as a whole number, in float64 where all
-// of a sum fits its 53 bits and in 64-bit integers beyond.  The order of additions then changes nothing, and the answer is the
-// real numbers' unless u lies within about 2^-40 of a border.  Float64 fused multiply-adds issue at the rate of float32 ones
-// here, so such a weight costs about 20 instructions.
+// of a sum fits its 53 bits and in 64-bit integers beyond.  The order of additions then changes nothing.  What is left are the
+// weights' own roundings, at most 2^-(F+1) of the largest each: the answer is the real numbers' unless u times the sum lies
+// within V 2^-(F+1) of a border (2^-36 at 512 logits, 2^-32 at 2048, 2^-28 at 131072; about sqrt(V) / V of that where the
+// roundings are of either sign; all of it where most logits are equal), next to which u itself is a multiple of 2^-24 or so.  A
+// weight below half a unit is 0: a filter that counts keeps it, and it is never drawn.  Float64 fused multiply-adds issue at
+// the rate of float32 ones here, so such a weight costs about 20 instructions.
 //
 // Every filter keeps a prefix of the row in falling order (ties by index), so their conjunction is the shortest of the
 // prefixes: one cut (a key, and how many of those that equal it).
