@@ -266,3 +266,23 @@ def test_weights_below_half_a_unit_are_never_drawn(ops, dev, V):
     for opt in (dict(), dict(top_k=10), dict(top_p=0.99), dict(top_k=10, min_p=1e-30)):
         ops.sample_tokens(logits, u, out, **opt)
         assert out.tolist() == [3, 3, 3], opt
+
+
+def test_decoder_code_of_a_column_without_a_number_to_draw(ops, dev):
+    """Where no logit of a column is a number above -inf the drawn code is -1; the other columns are what they are without it."""
+    from timeautodiff_amd import VAE
+    torch.manual_seed(3)
+    B, T, lat, nb, cards, nn = 3, 4, 4, 1, [5, 90], 2
+    F = nb + len(cards) + nn
+    ae = VAE.DeapStack(1, nb, len(cards), nn, cards, F, 24, 2, 16, 8, lat)
+    z, mask = torch.randn(B, T, lat, device=dev), torch.ones(B, T, F, device=dev)
+    u = torch.rand(len(cards), B, T, device=dev)
+    fine = ae.decode_to_tensor(z, mask, draw=dict(u=u))
+    assert bool((fine[..., nb:nb + 2] >= 0).all())
+    for number in (float("nan"), -float("inf")):
+        with torch.no_grad():
+            ae.get_parameter("cats_linears.0.bias").fill_(number)
+        got = ae.decode_to_tensor(z, mask, draw=dict(u=u))
+        assert bool((got[..., nb] == -1).all()) and bool((ae.decode_to_tensor(z, mask)[..., nb] == 0).all())
+        rest = [c for c in range(F) if c != nb]
+        assert torch.equal(got[..., rest], fine[..., rest])

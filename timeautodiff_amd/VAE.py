@@ -107,7 +107,8 @@ class DeapStack(nn.Module):
 
         draw (no counterpart in the reference): a dict of temperature, top_k, top_p, min_p (all optional, see
         ops.sample_tokens) and u, [n_cats, B, T] uniform numbers in [0, 1) (default: drawn on the device by torch's
-        generator): the categorical codes are drawn from the decoder's distributions instead of taken as their argmax."""
+        generator): the categorical codes are drawn from the decoder's distributions instead of taken as their argmax.
+        A code is -1 where no logit of its column is a number above -inf (the argmax gives 0 there)."""
         eng = self.engine(latent_feature.device if latent_feature.is_cuda else None)
         eng.fp.version += 1
         z = self._dev_f32(latent_feature, eng)
