@@ -178,6 +178,18 @@ def test_distill_loss_of_entries_on_masked_logits(ops, dev, dtype, V):
             assert np.all(np.abs(f64(d[r]) - grad[r]) <= tol), r
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [16, 17, 32, 33, 49, 128, 129, 256, 257, 512, 513, 1024, 1025, 16384, 16385, 32768, 32769])
+def test_distill_loss_where_its_forms_change(ops, dev, dtype, V):
+    from test_gpu_tokens import check_distill, distill_inputs
+    rng = np.random.default_rng(V)
+    for extra, offset in ((0, 0), (3, 1)):
+        logits, index, value = distill_inputs(5, V, 12, dtype, dev, rng, extra, offset)
+        index[1, 3] = index[1, 7]
+        check_distill(ops, dev, logits, index, value, 1.25, None, 0.5)
+        check_distill(ops, dev, logits, index, value, 1.25, None, 0.5, inplace=True)
+
+
 # ------------------------------------------------------------------ rows out of wider tensors
 @pytest.mark.parametrize("B,T,V", [(4, 5, 300), (3, 1, 40), (1, 6, 17)])
 def test_last_step_of_a_sequence(ops, dev, B, T, V):

@@ -281,10 +281,11 @@ __global__ __launch_bounds__(NT, NT == 512 ? 4 : 1) void distill_row_kernel(Args
 
 template <typename T>
 int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
-  // 4, 16 or 64 lanes a row, so that a lane has at most 16 logits; then, by the row's bytes, workgroups of 256 threads that hold
-  // it whole (16384 x 5000 bf16: 103 us; 512 threads: 119) or of 512: with 8 pieces a thread held up to 16 of them in all (65536
-  // bf16: 222 us against 236 with 24) or in float32, whose pieces are fewer logits, up to 8, beyond with 16 (4096 x 32001: 217
-  // against 259 with 8)
+  // 4, 16 or 64 lanes a row, so that a lane has at most 16 logits; then workgroups of 256 threads, which hold 8192 bf16 or 4096
+  // float32 logits (16384 x 5000 bf16, K = 64: 103 us; 512 threads: 119); beyond 16384 logits of 512 threads, in bf16 with 8
+  // pieces each as long as these hold the row (8192 x 32001, K = 64: 229 us; with 16: 242), then with 16 (4096 x 50001 bf16: 177;
+  // with 8: 187, 24: 185; 4096 x 32001 float32: 217; with 8: 259)
+  constexpr int MIDDLE = sizeof(T) == 2 ? 8 : 16;
 #define SHORT_(G, E) hipLaunchKernelGGL((distill_short_kernel<T, G, E>), dim3((unsigned)cdiv64(A.rows, 256 / G)), dim3(256), 0, s, A, x, d)
 #define ROW_(NT, H) hipLaunchKernelGGL((distill_row_kernel<T, NT, H>), dim3((unsigned)A.rows), dim3(NT), 0, s, A, x, d)
   if (A.V <= 16) SHORT_(4, 4);
@@ -296,7 +297,7 @@ int launch_distill(const Args& A, const T* x, T* d, hipStream_t s) {
   else if (A.V <= 512) SHORT_(64, 8);
   else if (A.V <= 1024) SHORT_(64, 16);
   else if (A.V <= 16384) ROW_(256, 4);
-  else if (A.V <= (sizeof(T) == 2 ? 65536 : 16384)) ROW_(512, 8);
+  else if (A.V <= 32768) ROW_(512, MIDDLE);
   else ROW_(512, 16);
 #undef SHORT_
 #undef ROW_
