@@ -147,8 +147,8 @@ __global__ __launch_bounds__(1024) void sort_rank_kernel(int n, int64_t vocab, c
 // More: by digits of up to 9 bits from the lowest, two launches a digit.  A workgroup has a tile of neighbouring keys, every
 // wave a contiguous share of it, so that keys of one digit keep their order: the first launch counts digits by tile, the
 // second adds up what comes before (lower digits; earlier tiles; earlier waves) and moves the keys.  No workgroup waits for
-// another, and no distribution of tokens is worse than another.  98304 tokens of 9 bits: 3.2 + 9.5 us, latency of 48 to 96
-// workgroups (tiles of a quarter to a half of that number are slower, more of them read more counts).
+// another, and no distribution of tokens is worse than another.  98304 tokens of 9 bits: 3.2 + 9.5 us, latency of 96
+// workgroups (fewer and larger tiles are slower, more of them read more counts).
 constexpr int MAX_BINS = 512, MAX_TILES = 128, RWAVES = 8;
 
 struct Digit {
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
                                                                  float* __restrict__ dtable, int64_t ldg, float* __restrict__ part) {
   constexpr int CT = 64 * VEC * M, U = 8;
   __shared__ __attribute__((aligned(16))) float edge[GW][2][CT];
-  __shared__ uint32_t head_tok[GW], tail_tok[GW], state[GW];       // state: 1 a run came in, 2 and ends here, 4 one goes on
+  __shared__ uint32_t head_tok[GW], state[GW];       // state: 1 a run came in, 2 and ends here, 4 one goes on
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (blockIdx.x >= nchunks * ctiles) {
     // rows that no token names are zero (overwriting mode): a lane looks one row up in the sorted keys
@@ -355,10 +355,7 @@ __global__ __launch_bounds__(GW * 64) void embed_grad_sum_kernel(int64_t n, int 
       for (int p = 0; p < M; ++p) store_pack<float, VEC>(&edge[wave][came ? 0 : 1][(p * 64 + lane) * VEC], acc[p]);
       st |= came ? 1 : 4;
     }
-    if (lane == 0) {
-      head_tok[wave] = tok0;
-      tail_tok[wave] = __builtin_amdgcn_readlane(tok, live > 0 ? live - 1 : 0);
-    }
+    if (lane == 0) head_tok[wave] = tok0;
   }
   if (lane == 0) state[wave] = st;
   __syncthreads();
