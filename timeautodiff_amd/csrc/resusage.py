@@ -1,13 +1,14 @@
 #!/usr/bin/env python3
 """Print a per-kernel table (VGPRs, spills, scratch, LDS, occupancy) for one .hip file.
 usage: python resusage.py rnn.hip"""
+import os
 import re
 import subprocess
 import sys
 
 src = sys.argv[1]
-cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
-       "-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", "/tmp/_resusage.o"]
+flags = subprocess.run(["make", "-s", "-C", os.path.dirname(os.path.abspath(__file__)), "show-flags"], capture_output=True, text=True, check=True)
+cmd = ["/opt/rocm/bin/hipcc", *flags.stdout.split(), "-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", "/tmp/_resusage.o"]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr
 rows = []
 cur = None
