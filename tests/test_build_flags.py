@@ -25,3 +25,13 @@ def test_every_kernel_is_compiled_without_packed_float32():
     flags = make("show-flags")
     at = flags.index("-packed-fp32-ops")
     assert flags[at - 3:at] == ["-Xclang", "-target-feature", "-Xclang"] and "--offload-arch=gfx950" in flags
+
+
+def test_build_compiles_every_source_again(monkeypatch):
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
+    entry.build()
+    assert len(calls) == 1
+    plan = subprocess.run(calls[0] + ["-n"], capture_output=True, text=True, check=True).stdout
+    assert all(f" -c {f} " in plan for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
