@@ -32,6 +32,7 @@ def test_build_compiles_every_source_again(monkeypatch):
     calls = []
     monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
     entry.build()
+    monkeypatch.undo()
     assert len(calls) == 1
     plan = subprocess.run(calls[0] + ["-n"], capture_output=True, text=True, check=True).stdout
     assert all(f" -c {f} " in plan for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
