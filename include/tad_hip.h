@@ -594,7 +594,8 @@ int tad_token_embed_bwd(int64_t n, int D, int64_t vocab, const int64_t* tokens, 
  * both).  dlogits may be NULL
  * (the loss alone) or the logits' own storage (same row stride).  Statistics and sums are float32.  The loss and the gradient
  * of a row are 0 where its weight is 0 (whatever else it holds), where it has no entry with a value above -inf, and where no
- * student logit is above -inf.  A logit of -inf has p = 0; q above 0 there makes the row's loss +inf. */
+ * student logit is above -inf.  A logit of -inf has p = 0; q above 0 there makes the row's loss +inf.  A logit
+ * masked with the type's lowest value has p = 0 too, and q there the finite loss of the formula (+inf only past float32's range). */
 int tad_distill_loss(int64_t rows, int64_t V, int K, const void* logits, int dtype, int64_t ld, const int64_t* index, const float* value,
                      int64_t ld_t, float tau, const float* row_weight, float grad_scale, float* loss_rows, void* dlogits, int64_t ldd,
                      tad_stream_t stream);
